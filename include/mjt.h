@@ -432,6 +432,52 @@ int mjt_fused_reindex_reduce_then(const mjt_fused_desc* desc, const mjt_tensor* 
                                   int n_overflow_conditions, const char* const* overflow_conditions, int n_extras, const mjt_tensor* extras,
                                   const mjt_fused_desc* behind);
 
+/* ---- operators of transformer layers ------------------------------------
+ * What stands around attention and the linear layers (kernels/dropout.h,
+ * head_norm_rope.h, gated_*.h hold the formulas).  bfloat16, float16 and
+ * float32; computed in 32 bits, 16-bit results are rounded to nearest even.
+ * A NULL result is one that is not wanted. */
+
+/* y = residual + (keep ? x / (1 - p) : 0), residual NULL: without.  keep(e)
+ * depends on the element's place, the key and the call's number alone
+ * (MJT_VAR_SCALAR vars whose ivalue holds 64 bits), so that the gradient is
+ * the same call on dy with residual NULL. */
+int mjt_dropout(const mjt_tensor* x, const mjt_tensor* residual, const mjt_tensor* y, double p, const mjt_fused_var* key, const mjt_fused_var* call);
+
+/* x [.., tokens, heads, dim] with the heads of queries, keys and values side
+ * by side: q and k are normalised by the root of their mean square for each
+ * head, scaled, and turned by their positions; v is copied.  q, k, v are
+ * [.., tokens, heads, dim] or, heads_first, [.., heads, tokens, dim].  Scales
+ * of dim elements, both or none (no norm).  table: float32 [positions, pairs,
+ * 2], cosine and sine (NULL: no rotation); pairs are neighbours (interleaved)
+ * or elements i and i + pairs.  positions: int32, one for every token or for
+ * every token of a sequence, for each axis (NULL: 0, 1, .. along a sequence).
+ * A position outside the table turns into NaN. */
+#define MJT_MOST_AXES 8
+typedef struct {
+    int32_t q_heads, k_heads, v_heads;
+    int32_t interleaved, heads_first;
+    int32_t n_axes;                       /* 0: one, for all pairs */
+    int32_t sections[MJT_MOST_AXES];      /* pairs of each axis */
+    double  eps;
+} mjt_head_norm;
+int mjt_head_norm_rope(const mjt_tensor* x, const mjt_tensor* q_scale, const mjt_tensor* k_scale, const mjt_tensor* table, const mjt_tensor* positions,
+                       const mjt_head_norm* p, const mjt_tensor* q, const mjt_tensor* k, const mjt_tensor* v);
+/* Its gradient: dq, dk, dv as above (NULL: zero). */
+int mjt_head_norm_rope_grad(const mjt_tensor* x, const mjt_tensor* q_scale, const mjt_tensor* k_scale, const mjt_tensor* table, const mjt_tensor* positions,
+                            const mjt_head_norm* p, const mjt_tensor* dq, const mjt_tensor* dk, const mjt_tensor* dv, const mjt_tensor* dx,
+                            const mjt_tensor* dq_scale, const mjt_tensor* dk_scale);
+
+/* y[rows, f] = act(x g^T) * (x u^T) for weights w[2 f, k] = g above u;
+ * activation 0 silu, 1 gelu (by the normal distribution), 2 relu, 3 sigmoid.
+ * both: float32 [rows, 2 f], the two products themselves, which the gradient
+ * reads.  mjt_gated_linear_grad makes d[rows, 2 f], the gradient of `both`, in
+ * dy's dtype; then dx = d w and dw = d^T x are products: mjt_matmul_nearest,
+ * which is mjt_matmul with bfloat16 results rounded to nearest even. */
+int mjt_gated_linear(const mjt_tensor* x, const mjt_tensor* w, int activation, const mjt_tensor* y, const mjt_tensor* both);
+int mjt_gated_linear_grad(const mjt_tensor* dy, const mjt_tensor* both, int activation, const mjt_tensor* d);
+int mjt_matmul_nearest(const mjt_tensor* a, const mjt_tensor* b, const mjt_tensor* c, int trans_a, int trans_b);
+
 /* ---- index-expression helper ------------------------------------------
  * Parses one index expression (the language of opt/expr.h:38-143 restricted
  * to what ops/reindex_op.h:58-68 allows) and, when it is affine in i0..i9

@@ -18,6 +18,7 @@ from .core import (Var, array, unary, binary, ternary, broadcast, broadcast_var,
 from .executor import run_sync, stats as executor_stats
 from .flags import flags, flag_scope
 from . import dtypes
+from . import layers
 from . import nn
 from .grad import grad
 from . import misc
@@ -71,6 +72,7 @@ _rng = [np.random.default_rng(0)]
 
 def set_seed(seed):
     _rng[0] = np.random.default_rng(seed)
+    layers.generator.seed(seed)
 
 
 def random(shape, dtype="float32", type="uniform"):

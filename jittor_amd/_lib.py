@@ -85,6 +85,16 @@ class ConvParams(ctypes.Structure):
                 ("dil_h", ctypes.c_int32), ("dil_w", ctypes.c_int32)]
 
 
+class HeadNorm(ctypes.Structure):
+    _fields_ = [("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32), ("v_heads", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("heads_first", ctypes.c_int32), ("n_axes", ctypes.c_int32),
+                ("sections", ctypes.c_int32 * 8), ("eps", ctypes.c_double)]
+
+
+MOST_AXES = 8
+ACTIVATIONS = ["silu", "gelu", "relu", "sigmoid"]
+
+
 # every symbol include/mjt.h declares
 EXPORTS = ["mjt_init", "mjt_shutdown", "mjt_last_error", "mjt_get_device_info",
            "mjt_dtype_name", "mjt_op_name", "mjt_dtype_from_name", "mjt_op_from_name",
@@ -94,6 +104,7 @@ EXPORTS = ["mjt_init", "mjt_shutdown", "mjt_last_error", "mjt_get_device_info",
            "mjt_fused_elementwise", "mjt_fused_reduce", "mjt_fused_rows", "mjt_conv2d_meta", "mjt_conv2d_meta_pack", "mjt_conv2d_meta_packed", "mjt_conv2d_meta_grouped", "mjt_conv2d_meta_dgrad", "mjt_conv2d_meta_dgrad_depthwise", "mjt_conv2d_meta_wgrad", "mjt_conv2d_meta_wgrad_grouped",
            "mjt_reindex_then_reduce", "mjt_fused_reindex_reduce", "mjt_matmul", "mjt_matmul_available",
            "mjt_conv2d_meta_backward_depthwise", "mjt_conv2d_meta_then", "mjt_conv2d_meta_dgrad_then", "mjt_matmul_then", "mjt_fused_reindex_reduce_then",
+           "mjt_dropout", "mjt_head_norm_rope", "mjt_head_norm_rope_grad", "mjt_gated_linear", "mjt_gated_linear_grad", "mjt_matmul_nearest",
            "mjt_expr_affine", "mjt_where_count", "mjt_where",
            "mjt_record_begin", "mjt_record_end", "mjt_record_relocate", "mjt_record_launch", "mjt_record_free",
            "mjt_jit_stats", "mjt_last_kernel"]
@@ -164,6 +175,13 @@ def load():
     lib.mjt_conv2d_meta_dgrad_then.argtypes = lib.mjt_conv2d_meta_dgrad.argtypes + [ctypes.POINTER(FusedDesc)]
     lib.mjt_fused_reindex_reduce_then.argtypes = lib.mjt_fused_reindex_reduce.argtypes + [ctypes.POINTER(FusedDesc)]
     lib.mjt_matmul_then.argtypes = lib.mjt_matmul.argtypes + [ctypes.POINTER(FusedDesc)]
+    t = ctypes.POINTER(Tensor)
+    lib.mjt_dropout.argtypes = [t, t, t, ctypes.c_double, ctypes.POINTER(FusedVar), ctypes.POINTER(FusedVar)]
+    lib.mjt_head_norm_rope.argtypes = [t] * 5 + [ctypes.POINTER(HeadNorm)] + [t] * 3
+    lib.mjt_head_norm_rope_grad.argtypes = [t] * 5 + [ctypes.POINTER(HeadNorm)] + [t] * 6
+    lib.mjt_gated_linear.argtypes = [t, t, ctypes.c_int, t, t]
+    lib.mjt_gated_linear_grad.argtypes = [t, t, ctypes.c_int, t]
+    lib.mjt_matmul_nearest.argtypes = lib.mjt_matmul.argtypes
     lib.mjt_where_count.argtypes = [ctypes.POINTER(Tensor), ctypes.POINTER(ctypes.c_int64)]
     lib.mjt_where.argtypes = [ctypes.POINTER(Tensor), ctypes.c_int64, ctypes.POINTER(Tensor)]
     lib.mjt_expr_affine.argtypes = [ctypes.c_char_p, ctypes.POINTER(Tensor), ctypes.POINTER(Tensor),

@@ -312,6 +312,20 @@ class ReindexReduceOp(Op):
         return ("reindex_reduce", self.op, tuple(self.indexes), tuple(self.overflow_conditions))
 
 
+class KernelOp(Op):
+    """One of the results of a library call that may have several (layers.py).  The ops of one call share `call`, what is called and with
+    which options, and read the same inputs; whichever of them are pending together run as one launch, and the gradients of all of
+    them are taken together."""
+    kind = "kernel"
+
+    def __init__(self, inputs, call, index):
+        Op.__init__(self, inputs)
+        self.call, self.index = call, index
+
+    def sig(self):
+        return ("kernel", self.call.key(), self.index)
+
+
 # --------------------------------------------------------------------------
 # Var
 # --------------------------------------------------------------------------

@@ -3,7 +3,9 @@
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>
+#include <algorithm>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -199,6 +201,20 @@ std::string fused_op_expr(const mjt_fused_desc* d, const mjt_fused_op& o);
 
 inline uint64_t bits_of(double v) { uint64_t u; memcpy(&u, &v, 8); return u; }
 inline uint64_t bits_of_ptr(const void* p) { return (uint64_t)(uintptr_t)p; }
+
+// While one of these lives on this thread, products write bfloat16 results rounded to nearest even instead of truncated (op_matmul.cpp).
+struct Nearest {
+    Nearest();
+    ~Nearest();
+    static bool on();
+};
+
+// ---- operators of transformer layers (op_layers.cpp) ----
+// The number of a float type inside kernels/element.h, -1 for other types.
+int element_type(int dtype);
+// The kernel `name` made of embedded source files behind `defines`, built once; its launcher is called for every launch, so the key is
+// all there is to look up.
+JitKernel* layer_kernel(const std::string& name, std::initializer_list<const char*> files, const std::string& defines);
 
 // Threads of a workgroup of kernels/gemm_mfma.h, with float32 operands in parts or as they are.
 inline unsigned product_threads(bool split) { return split ? 512 : 256; }

@@ -2,7 +2,7 @@
 // group behind the product (epilogue.h).
 //
 // Supplied by the host: SLICES (at most 16), VS (adjacent results a lane takes: 4, 2 or 1), OUT (0 bfloat16 by truncation, 1 float16 rounded
-// to nearest even, 2 float32).  a[0] part, a[1] y, a[2] vectors of VS.
+// to nearest even, 2 float32, 3 bfloat16 rounded to nearest even).  a[0] part, a[1] y, a[2] vectors of VS.
 //
 // Bound by the trip to memory: the parts lie in the caches that the product has just written them to.  All of a lane's loads are under way
 // together; the slices are added in their order.  us, the general reduce (and the group by itself) / this: 9 slices of 4 x 64 x 14 x 14 3.3 /
@@ -40,6 +40,8 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
     for (int k = 0; k < VS; k++)
 #if OUT == 0
         o.v[k] = (unsigned short)(__float_as_uint(sum.v[k]) >> 16);                    // truncation (type/fp16_compute.h:238-241)
+#elif OUT == 3
+        o.v[k] = __builtin_bit_cast(unsigned short, (__bf16)sum.v[k]);
 #else
         o.v[k] = __builtin_bit_cast(unsigned short, (_Float16)sum.v[k]);                // nearest even (type/fp16_compute.h:147-198)
 #endif

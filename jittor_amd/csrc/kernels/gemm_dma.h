@@ -8,7 +8,7 @@
 // products and float32 accumulation.
 //
 // Supplied by the host: VS (adjacent results a lane stores: 4, 2 or 1), IN (0 bfloat16, 1 float16), OUT (0 bfloat16 by truncation, 1 float16 rounded to
-// nearest even, 2 float32), A_KCONT, B_KCONT (the operand's memory has k innermost).  K is a multiple of 64, leading
+// nearest even, 2 float32, 3 bfloat16 rounded to nearest even), A_KCONT, B_KCONT (the operand's memory has k innermost).  K is a multiple of 64, leading
 // dimensions are multiples of 16 bytes and the operand pointers 16-byte aligned (the host sends everything else to the
 // general kernel).
 //
@@ -385,6 +385,8 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
                 for (int k = 0; k < VS; k++)
 #if OUT == 0
                     o.v[k] = (unsigned short)(__float_as_uint(r.v[k]) >> 16);     // truncation (type/fp16_compute.h:238-241)
+#elif OUT == 3
+                    o.v[k] = __builtin_bit_cast(unsigned short, (__bf16)r.v[k]);
 #else
                     o.v[k] = __builtin_bit_cast(unsigned short, (_Float16)r.v[k]);                // nearest even (type/fp16_compute.h:147-198)
 #endif
@@ -418,6 +420,8 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
                     ((float*)p.a[2])[at] = v;
 #elif OUT == 0
                     ((unsigned short*)p.a[2])[at] = (unsigned short)(__float_as_uint(v) >> 16);     // truncation (type/fp16_compute.h:238-241)
+#elif OUT == 3
+                    ((unsigned short*)p.a[2])[at] = __builtin_bit_cast(unsigned short, (__bf16)v);
 #else
                     ((unsigned short*)p.a[2])[at] = __builtin_bit_cast(unsigned short, (_Float16)v);     // nearest even (type/fp16_compute.h:147-198)
 #endif

@@ -8,7 +8,7 @@
 // and float32 accumulation, or float32 throughout.
 //
 // Supplied by the host: IN (0 bfloat16, 1 float16, 2 float32), OUT (0 bfloat16 by
-// truncation, 1 float16 rounded to nearest even, 2 float32), MI, NI (32x32 accumulator
+// truncation, 1 float16 rounded to nearest even, 2 float32, 3 bfloat16 rounded to nearest even), MI, NI (32x32 accumulator
 // tiles per wave along m and n), A_KCONT, B_KCONT (the operand's memory has k innermost).
 //
 // Mapping.  A workgroup of four waves (2 x 2; SPLIT: eight) owns a TM x TN = 64 MI x 64 NI tile of C and
@@ -770,6 +770,8 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
                     ((float*)p.a[2])[at] = v;
 #elif OUT == 0
                     ((unsigned short*)p.a[2])[at] = (unsigned short)(__float_as_uint(v) >> 16);     // truncation (type/fp16_compute.h:238-241)
+#elif OUT == 3
+                    ((unsigned short*)p.a[2])[at] = __builtin_bit_cast(unsigned short, (__bf16)v);
 #else
                     const _Float16 h = (_Float16)v;                        // nearest even (type/fp16_compute.h:147-198)
                     ((unsigned short*)p.a[2])[at] = __builtin_bit_cast(unsigned short, h);

@@ -2,7 +2,8 @@
 // (float64, leading dimensions or pointers that are not multiples of 16 bytes):
 //   C[b][M][N] = sum_k A'[b][M][K] * B'[b][K][N]
 // A workgroup of 256 lanes owns a 64 x 64 tile of C, a lane 4 x 4 of it; K in stages of 16 through LDS.
-// Supplied by the host: TIN, TOUT (element types), TACC (float, or double for float64), A_KCONT, B_KCONT.
+// Supplied by the host: TIN, TOUT (element types), TACC (float, or double for float64), A_KCONT, B_KCONT, NEAREST (bfloat16 results
+// rounded to nearest even; otherwise truncated).
 struct Params { void* a[12]; };   // as in kernels/gemm_mfma.h
 
 __device__ __forceinline__ TACC mjt_to_acc(double v) { return (TACC)v; }
@@ -60,6 +61,10 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int row = m0 + ty * 4 + i, col = n0 + tx * 4 + j;
+#if NEAREST
+            if (row < M && col < N) C[(long long)row * ldc + col].x = __builtin_bit_cast(unsigned short, (__bf16)acc[i][j]);
+#else
             if (row < M && col < N) C[(long long)row * ldc + col] = (TOUT)acc[i][j];
+#endif
         }
 }

@@ -44,6 +44,7 @@ void remember(const std::string& key, JitKernel* k) {
     std::lock_guard<std::mutex> lock(g_mu);
     g_kernels.emplace(key, k);
 }
+thread_local int t_nearest = 0;
 int env_int(const char* name, int dflt) {
     const char* v = getenv(name);
     return v && *v ? atoi(v) : dflt;
@@ -69,6 +70,10 @@ const void* padded_rows(int which, const void* src, int dtype, int64_t rows, int
     return d.ptr;
 }
 }  // namespace
+
+Nearest::Nearest() { t_nearest++; }
+Nearest::~Nearest() { t_nearest--; }
+bool Nearest::on() { return t_nearest > 0; }
 
 // One strided-batched product C[b] = A'[b] * B'[b] over plain pointers: M x K times K x N, leading dimensions and
 // batch strides in elements (a batch stride of 0 shares the operand).  a_kcont / b_kcont: the operand's memory has
@@ -114,7 +119,7 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
         if (tile) {
             const int64_t tm = (M + tile - 1) / tile, tn = (N + tile - 1) / tile;
             const int in = in_dtype == MJT_BFLOAT16 ? 0 : 1;
-            const int out = out_dtype == MJT_BFLOAT16 ? 0 : out_dtype == MJT_FLOAT16 ? 1 : 2;
+            const int out = out_dtype == MJT_BFLOAT16 ? Nearest::on() ? 3 : 0 : out_dtype == MJT_FLOAT16 ? 1 : 2;
             // a short sum on 128 x 128 tiles: two stage buffers, so that a compute unit holds two workgroups and one
             // computes or stores while the other waits for its operands
             // 128 x 128 tiles: with more tiles than compute units two stage buffers, so that a compute unit holds two
@@ -133,7 +138,7 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
             if (!k) {
                 std::ostringstream name;
                 name << "mjt_gemm_mfma_" << mjt_dtype_name(in_dtype) << "_" << mjt_dtype_name(out_dtype) << "_" << tile << "x" << tile << (a_kcont ? "_n" : "_t")
-                     << (b_kcont ? "t" : "n") << "_direct" << (wpe == 2 ? "2" : "") << ep.suffix();
+                     << (b_kcont ? "t" : "n") << "_direct" << (wpe == 2 ? "2" : "") << (out == 3 ? "_nearest" : "") << ep.suffix();
                 std::ostringstream src;
                 src << ep.defs << "#define VS " << vs << "\n#define ENTRY " << name.str() << "\n#define IN " << in << "\n#define OUT " << out << "\n#define A_KCONT " << (a_kcont ? 1 : 0)
                     << "\n#define B_KCONT " << (b_kcont ? 1 : 0) << "\n#define TILE " << tile << "\n#define NBUF " << nbuf << "\n#define WPE " << wpe << "\n";
@@ -217,7 +222,7 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
         if (!part_mem) slices = 1;
         const int MI = best_mi, NI = best_ni;
         const int in = in_dtype == MJT_BFLOAT16 ? 0 : in_dtype == MJT_FLOAT16 ? 1 : 2;
-        const int out = slices > 1 || out_dtype == MJT_FLOAT32 ? 2 : out_dtype == MJT_BFLOAT16 ? 0 : 1;
+        const int out = slices > 1 || out_dtype == MJT_FLOAT32 ? 2 : out_dtype == MJT_BFLOAT16 ? Nearest::on() ? 3 : 0 : 1;
         const bool one_stage = stages == 1 && !getenv("MJT_GEMM_TWO_BUFFERS");       // a single stage of the kernel's k loop
         const EpilogueCode ep = epilogue_code(1, 12, out_dtype, slices == 1 && ldc == N && (batch == 1 || sc == M * N) ? M * N * batch : -1);
         std::ostringstream key;
@@ -226,7 +231,7 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
         if (!k) {
             std::ostringstream name;
             name << "mjt_gemm_mfma_" << mjt_dtype_name(in_dtype) << "_" << (out == 2 ? "float32" : mjt_dtype_name(out_dtype)) << "_" << 64 * MI << "x" << 64 * NI
-                 << (a_kcont ? "_n" : "_t") << (b_kcont ? "t" : "n") << (one_stage ? "_k1" : "") << (split ? "_parts" : "") << (slices > 1 ? "_slices" : "") << ep.suffix();
+                 << (a_kcont ? "_n" : "_t") << (b_kcont ? "t" : "n") << (one_stage ? "_k1" : "") << (split ? "_parts" : "") << (slices > 1 ? "_slices" : "") << (out == 3 ? "_nearest" : "") << ep.suffix();
             std::ostringstream src;
             src << ep.defs << "#define NBUF " << (one_stage ? 1 : 2) << "\n#define SLICED " << (slices > 1 ? 1 : 0) << "\n#define SPLIT " << (split ? 1 : 0) << "\n";
             src << "#define ENTRY " << name.str() << "\n#define IN " << in << "\n#define OUT " << out << "\n#define MI " << MI
@@ -259,15 +264,16 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
         return;
     }
     std::ostringstream key;
-    key << "gemmp|" << in_dtype << "|" << out_dtype << a_kcont << b_kcont;
+    const bool nearest = out_dtype == MJT_BFLOAT16 && Nearest::on();
+    key << "gemmp|" << in_dtype << "|" << out_dtype << a_kcont << b_kcont << nearest;
     JitKernel* k = cached(key.str());
     if (!k) {
         std::ostringstream name;
-        name << "mjt_gemm_plain_" << mjt_dtype_name(in_dtype) << "_" << mjt_dtype_name(out_dtype) << (a_kcont ? "_n" : "_t") << (b_kcont ? "t" : "n");
+        name << "mjt_gemm_plain_" << mjt_dtype_name(in_dtype) << "_" << mjt_dtype_name(out_dtype) << (a_kcont ? "_n" : "_t") << (b_kcont ? "t" : "n") << (nearest ? "_nearest" : "");
         std::ostringstream src;
         src << "#define ENTRY " << name.str() << "\n#define TIN " << dtype_cname(in_dtype) << "\n#define TOUT " << dtype_cname(out_dtype)
             << "\n#define TACC " << (in_dtype == MJT_FLOAT64 ? "double" : "float") << "\n#define A_KCONT " << (a_kcont ? 1 : 0)
-            << "\n#define B_KCONT " << (b_kcont ? 1 : 0) << "\n";
+            << "\n#define B_KCONT " << (b_kcont ? 1 : 0) << "\n#define NEAREST " << (nearest ? 1 : 0) << "\n";
         src << embedded_source("prelude.h") << "\n" << embedded_source("gemm_plain.h") << "\n";
         k = jit_get(src.str(), name.str());
         remember(key.str(), k);

@@ -23,7 +23,7 @@ SliceFold::SliceFold(const void* part, void* y, int dtype, int64_t n, int64_t sl
     while (vs > 1 && (n % vs || (uintptr_t)y % (size_t)(vs * osz))) vs /= 2;
     ep = epilogue_code(vs, 3, dtype, n);
     if (!ep.on) check_no_epilogue();                              // (before anything is launched)
-    const int out = dtype == MJT_BFLOAT16 ? 0 : dtype == MJT_FLOAT16 ? 1 : 2;
+    const int out = dtype == MJT_BFLOAT16 ? Nearest::on() ? 3 : 0 : dtype == MJT_FLOAT16 ? 1 : 2;
     std::ostringstream key;
     key << out << vs << "," << slices << ep.key;
     {
@@ -33,7 +33,7 @@ SliceFold::SliceFold(const void* part, void* y, int dtype, int64_t n, int64_t sl
     }
     if (!k) {
         std::ostringstream name;
-        name << "mjt_fold_slices_" << mjt_dtype_name(dtype) << "_" << slices << "v" << vs << ep.suffix();
+        name << "mjt_fold_slices_" << mjt_dtype_name(dtype) << "_" << slices << "v" << vs << (out == 3 ? "_nearest" : "") << ep.suffix();
         k = jit_get(ep.defs + "#define ENTRY " + name.str() + "\n#define SLICES " + std::to_string(slices) + "\n#define VS " + std::to_string(vs) + "\n#define OUT " +
                         std::to_string(out) + "\n" + embedded_source("fold_slices.h") + "\n", name.str());
         std::lock_guard<std::mutex> lock(g_mu);

@@ -37,7 +37,7 @@ struct Ref {
 PyObject* keep(PyObject* p) { Py_XINCREF(p); return p; }
 
 #define NAMES(X) X(shape) X(num) X(dtype) X(_op) X(_history) X(id) X(_out_ref) X(inputs) X(amp) X(op) X(bcast_mask) X(keepdims_mask) X(reduce_mask) X(is_scalar) \
-    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) \
+    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) X(call) X(index) \
     X(_binary_dtypes) X(binary_dtype_infer) X(unary_dtype_infer) X(reduce_dtype_infer) X(dtype_infer) X(cast) X(add) X(mean) X(float16) X(bfloat16) X(float32)
 #define DECLARE(n) PyObject* s_##n;
 NAMES(DECLARE)
@@ -760,6 +760,7 @@ bool backward(PyObject* loss, const std::vector<std::pair<long long, Ref>>& orde
         if (fold && PySet_Add(ones, own(seed, s_id))) return false;
     }
     PyObject* dt = PyModule_GetDict(g_dt);
+    std::unordered_set<PyObject*> calls;                       // those whose gradients have been taken
     for (size_t q = order.size(); q-- > 0;) {
         PyObject* v = order[q].second.p;
         auto it = grads->find(order[q].first);
@@ -767,10 +768,55 @@ bool backward(PyObject* loss, const std::vector<std::pair<long long, Ref>>& orde
         if (it == grads->end() || !h || h == Py_None) continue;
         Ref g(keep(it->second.p)), history(keep(h));
         PyObject *op = PyTuple_GET_ITEM(h, 0), *inputs = PyTuple_GET_ITEM(h, 1);
+        auto add = [&](PyObject* u, Ref du) {                  // a contribution to the gradient of u
+            Shape ds, us;
+            if (!var_shape(du.p, &ds) || !var_shape(u, &us)) return false;
+            if (!(ds == us)) {
+                Ref a(shape_list(ds)), b(shape_list(us));
+                if (a && b) PyErr_Format(PyExc_RuntimeError, "gradient of %R has shape %R, expected %R", op, a.p, b.p);
+                return false;
+            }
+            const long long uid = id_of(u);
+            auto at = grads->find(uid);
+            if (at == grads->end()) {
+                grads->emplace(uid, std::move(du));
+                return true;
+            }
+            PyObject* sum = binary(at->second.p, du.p, s_add);
+            if (!sum) return false;
+            grads->find(uid)->second = Ref(sum);
+            return true;
+        };
+        // The results of one call: their gradients go through it together, at the first of them that has one.  They are made one after
+        // the other, so whatever reads any of them has a greater id than all, and no gradient of theirs still grows.
+        if (PyObject* call = own(op, s_call)) {
+            if (!calls.insert(call).second) continue;
+            Ref douts(PyDict_New()), wanted(PyList_New(0));
+            if (!douts || !wanted) return false;
+            for (auto& [id, u] : order) {
+                PyObject* uh = own(u.p, s__history);
+                auto found = grads->find(id);
+                if (!uh || uh == Py_None || found == grads->end() || own(PyTuple_GET_ITEM(uh, 0), s_call) != call) continue;
+                PyObject* index = own(PyTuple_GET_ITEM(uh, 0), s_index);
+                if (!index || PyDict_SetItem(douts.p, index, found->second.p)) return false;
+            }
+            for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(inputs); i++) {
+                PyObject* u = PyTuple_GET_ITEM(inputs, i);
+                Ref type = attr(u, s_dtype);
+                if (!type || PyList_Append(wanted.p, dep.count(id_of(u)) && is_float_name(type.p) ? Py_True : Py_False)) return false;
+            }
+            Ref dus(PyObject_CallFunctionObjArgs(others, op, inputs, v, douts.p, wanted.p, nullptr));
+            if (!dus) return false;
+            if (!PyList_Check(dus.p) || PyList_GET_SIZE(dus.p) != PyTuple_GET_SIZE(inputs)) { PyErr_SetString(PyExc_TypeError, "a call's gradients are a list, one for each input"); return false; }
+            for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(inputs); i++) {
+                PyObject* du = PyList_GET_ITEM(dus.p, i);
+                if (du != Py_None && PyList_GET_ITEM(wanted.p, i) == Py_True && !add(PyTuple_GET_ITEM(inputs, i), Ref(keep(du)))) return false;
+            }
+            continue;
+        }
         for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(inputs); i++) {
             PyObject* u = PyTuple_GET_ITEM(inputs, i);
-            const long long uid = id_of(u);
-            if (!dep.count(uid)) continue;
+            if (!dep.count(id_of(u))) continue;
             Ref type = attr(u, s_dtype);
             if (!type) return false;
             if (!is_float_name(type.p)) continue;
@@ -790,20 +836,7 @@ bool backward(PyObject* loss, const std::vector<std::pair<long long, Ref>>& orde
             }
             if (!du) return false;
             if (du.p == Py_None) continue;
-            Shape ds, us;
-            if (!var_shape(du.p, &ds) || !var_shape(u, &us)) return false;
-            if (!(ds == us)) {
-                Ref a(shape_list(ds)), b(shape_list(us));
-                if (a && b) PyErr_Format(PyExc_RuntimeError, "gradient of %R has shape %R, expected %R", op, a.p, b.p);
-                return false;
-            }
-            auto at = grads->find(uid);
-            if (at == grads->end()) grads->emplace(uid, std::move(du));
-            else {
-                PyObject* sum = binary(at->second.p, du.p, s_add);
-                if (!sum) return false;
-                grads->find(uid)->second = Ref(sum);
-            }
+            if (!add(u, std::move(du))) return false;
         }
     }
     return true;

@@ -16,9 +16,10 @@ import threading
 from . import _graph
 from . import _lib
 from . import core
+from . import layers
 from . import rowfuse
 from .core import (Var, Buffer, UnaryOp, BinaryOp, TernaryOp, BroadcastOp,
-                   ReduceOp, ReindexOp, ReindexReduceOp)
+                   ReduceOp, ReindexOp, ReindexReduceOp, KernelOp)
 from ._lib import MjtError
 from . import profiler as _profiler
 from .flags import flags
@@ -1030,13 +1031,28 @@ def _execute(ops, target_ids):
         made = {op.out.id for op in members}
         return {u.id for op in members for u in ins(op)} - made
 
-    tasks = []
+    def run_call(ops):
+        timed(lambda: layers.launch(sys.modules[__name__], ops), ops[0].call.name, lambda: (sum(u.nbytes for u in ops[0].inputs), sum(op.out.nbytes for op in ops)))
+
+    tasks, same_task = [], {}
     for s in range(nstage):
         for members in by_stage_groups[s]:
             if id(members) not in absorbed_groups:
                 tasks.append(rowfuse.Task(lambda members=members: run_members(members), reads_of(members), {op.out.id for op in members}, members))
+        calls = []                                             # (results of one call, its inputs are the same objects: one stage)
         for op in by_stage_other[s]:
             if op.id in absorbed_nodes:
+                continue
+            if isinstance(op, KernelOp):
+                same = next((c for c in calls if c[0].call is op.call and all(a is b for a, b in zip(c[0].inputs, op.inputs))), None)
+                if same is not None:
+                    same.append(op)
+                    same_task[id(same)].writes.add(op.out.id)
+                    continue
+                calls.append([op])
+                t = rowfuse.Task(lambda ops=calls[-1]: run_call(ops), {u.id for u in op.inputs}, {op.out.id}, node=op)
+                same_task[id(calls[-1])] = t
+                tasks.append(t)
                 continue
             members, reads = prologue_of.get(op.id, ()), {u.id for u in op.inputs}
             if op.id in scatter_of:

@@ -13,7 +13,8 @@ does not depend on gets zeros.
 """
 from . import _graph
 from . import core
-from .core import (Var, UnaryOp, BinaryOp, ReduceOp, ReindexOp, ReindexReduceOp,
+from . import layers
+from .core import (Var, UnaryOp, BinaryOp, ReduceOp, ReindexOp, ReindexReduceOp, KernelOp,
                    unary, binary, ternary, make_number, reindex, reindex_reduce, array)
 
 
@@ -81,6 +82,8 @@ def _binary_grad(op, x, y, z, dout, index):
 
 
 def _op_grad(op, inputs, out, dout, index):
+    if isinstance(op, KernelOp):                        # all results and inputs of its call at once
+        return layers.gradients(op, inputs, out, dout, index)
     x = inputs[index]
     if isinstance(op, UnaryOp):
         return _unary_grad(op, inputs[0], out, dout)

@@ -4,6 +4,7 @@ with meta-operators exactly as the reference writes them
 import numpy as np
 
 from . import core
+from . import layers
 from .flags import flags, flag_scope
 
 
@@ -218,6 +219,59 @@ def linear(x, weight, bias=None):
     """x * weight^T + bias (python/jittor/nn.py: linear)."""
     y = matmul_transpose(x, weight)
     return y if bias is None else core.binary(y, bias, "add")
+
+
+# ---- operators of transformer layers (layers.py, kernels/*.h) ---------------------------------------------------------
+def dropout(x, p=0.5, is_train=False, seed=None, offset=None, residual=None):
+    """x with each element zeroed with probability p and the others divided by 1 - p (python/jittor/nn.py: dropout); x itself where
+    `is_train` is False.  With `residual`, a Var like x, the sum of the two in the same pass.
+
+    The mask is never stored: it depends on the elements' places, `seed` and `offset` (integers of 64 bits) alone, and the gradient works
+    it out again.  Calls of one program that are to be independent differ in one of the two; without a seed the generator of jt.set_seed
+    numbers the calls.  A dropped element is 0 whatever it held."""
+    return layers.dropout(x, p, is_train, seed, offset, residual)
+
+
+def rope_table(n, dim, base=10000.0):
+    """Cosine and sine of position * base ** (-2 i / dim) for n positions and the dim / 2 pairs of `dim` rotated elements: float32
+    [n, dim / 2, 2], worked out in 64 bits.  A program keeps one for all its layers."""
+    return layers.rope_table(n, dim, base)
+
+
+def qkv_norm_rope(qkv, heads, kv_heads, q_scale=None, k_scale=None, table=None, positions=None, sections=None, eps=1e-6, interleaved=False, heads_first=False):
+    """(q, k, v) from the joint projection qkv [.., tokens, heads + 2 * kv_heads, dim]: every head of the queries and keys divided by the
+    root of its mean square (plus eps) and scaled by q_scale or k_scale [dim], then turned by its position; the values as they are.
+
+    `table` (rope_table) holds the angles of its first 2 * table.shape[1] elements; pairs are elements i and i + table.shape[1], or
+    neighbours with `interleaved`.  `positions` (int32 [.., tokens] or [tokens]; 0, 1, .. where left out) are rows of the table; one outside makes
+    what it turns NaN.  For images and video `sections` gives the number of pairs for each axis, and positions [axes, .., tokens].
+    Without scales the heads are only turned, without a table only normalised.  Results are [.., tokens, heads, dim], or with `heads_first`
+    [.., heads, tokens, dim], as attention's products read them."""
+    if (q_scale is None) != (k_scale is None):
+        raise ValueError("qkv_norm_rope: scales for the queries and for the keys, or none")
+    if heads < 1 or kv_heads < 1:
+        raise ValueError("qkv_norm_rope: %r heads of queries, %r of keys and values" % (heads, kv_heads))
+    scales = None if q_scale is None else (q_scale, k_scale)
+    return tuple(layers.head_norm_rope("qkv_norm_rope", qkv, (heads, kv_heads, kv_heads), scales, table, positions, sections, eps, interleaved, heads_first))
+
+
+def head_norm_rope(x, scale=None, table=None, positions=None, sections=None, eps=1e-6, interleaved=False, heads_first=False):
+    """qkv_norm_rope for heads of one kind: x [.., tokens, heads, dim], queries or keys on their own."""
+    x = core._as_var(x)
+    if x.ndim < 3 or x.shape[-2] < 1:
+        raise ValueError("head_norm_rope: x has to be [.., tokens, heads, dim], got %s" % list(x.shape))
+    return layers.head_norm_rope("head_norm_rope", x, (x.shape[-2], 0, 0), None if scale is None else (scale, scale), table, positions, sections, eps, interleaved, heads_first)[0]
+
+
+def gated_linear(x, weight, activation="silu"):
+    """activation(x * g^T) * (x * u^T) for weight [2 f, k] = g above u: the first half of a gated feed-forward layer, both projections and
+    what follows them in one pass.  `activation`: silu, gelu, relu or sigmoid."""
+    return layers.gated_linear(x, weight, activation)
+
+
+def gated_ffn(x, w_in, w_out, activation="silu"):
+    """The whole feed-forward layer: gated_linear(x, w_in) * w_out^T, w_in [2 f, k], w_out [n, f]."""
+    return matmul_transpose(gated_linear(x, w_in, activation), w_out)
 
 
 core.Var.matmul = core.Var.__matmul__ = matmul

@@ -1,0 +1,443 @@
+"""Operators of transformer layers on the GPU against the plain forms in 64 bits (layers_plain.py).
+
+Tolerances: the result's own rounding (half a unit of its type), plus what 32-bit arithmetic may add: a bound derived for each operator
+from the magnitudes of what is summed, E = 2^-24 relative for each operation."""
+import numpy as np
+import pytest
+
+import jittor_amd as jt
+from jittor_amd import core
+from jittor_amd.dtypes import bf16_bits_to_f32
+import layers_plain as P
+from layers_plain import E, TINY, ULP
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["float32", "bfloat16", "float16"]
+
+
+def _make(rng, shape, dtype, scale=1.0, shift=0.0):
+    """(Var, its exact values)"""
+    raw, exact = P.to_type(rng.standard_normal(shape) * scale + shift, dtype)
+    return jt.from_storage(raw, dtype), exact
+
+
+def _got(v):
+    return v.numpy().astype(np.float64)
+
+
+def _check(got, want, bound, dtype, what):
+    """|got - want| within the rounding of the result and `bound`; what is not finite has to be the same."""
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    assert np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)]), what
+    off = np.abs(got - want)[fine]
+    allowed = (np.broadcast_to(bound, want.shape)[fine]) * (1 + ULP[dtype]) + ULP[dtype] * np.abs(want[fine]) + TINY[dtype]
+    worst = np.argmax(off - allowed) if off.size else 0
+    assert not off.size or (off <= allowed).all(), (what, off.flat[worst], allowed.flat[worst])
+
+
+# ---- dropout ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1,), (7,), (8,), (3, 5, 11), (2, 1024), (1, 4099)])
+@pytest.mark.parametrize("p", [0.5, 0.1, 0.999, 1.0, 1e-9])
+def test_dropout(gpu, dtype, shape, p):
+    rng = np.random.default_rng(len(shape))
+    (x, xe), (r, re), (g, ge) = (_make(rng, shape, dtype) for _ in range(3))
+    seed, offset = -3 * (1 << 60) + 5, (1 << 63) + 9
+    keep = P.kept(x.num, p, seed, offset).reshape(shape)
+    f = np.float64(np.float32(1.0 / (1.0 - p))) if p < 1 else 0.0
+    for residual in (None, r):
+        y = jt.nn.dropout(x, p, True, seed=seed, offset=offset, residual=residual)
+        grads = jt.grad((y * g).sum(), [x] + ([] if residual is None else [r]))
+        jt.sync([y] + grads)
+        add = 0.0 if residual is None else re
+        _check(_got(y), np.where(keep, xe * f, 0.0) + add, 2 * E * (np.abs(xe * f) + np.abs(add)), dtype, "y")
+        _check(_got(grads[0]), np.where(keep, ge * f, 0.0), 2 * E * np.abs(ge * f), dtype, "dx")
+        if residual is not None:
+            assert np.array_equal(_got(grads[1]), ge)
+
+
+def test_dropout_at_the_threshold(gpu):
+    """p between two multiples of 2^-16: the lower halves of the numbers decide for one element in 65536, and have to."""
+    n = 1 << 17
+    u = P.numbers(n, 11, 2)
+    at = u[np.argsort(np.abs(u.astype(np.int64) - (1 << 31)))[:64]]
+    x = jt.array(np.ones(n, np.float32))
+    for t in sorted({int(v) + d for v in at[:6] for d in (0, 1)}):
+        y = jt.nn.dropout(x, t / 2.0 ** 32, True, seed=11, offset=2)
+        assert np.array_equal(_got(y) != 0, u >= t), t
+
+
+def test_dropped_infinities_and_nan_are_zero(gpu):
+    n, p = 4096, 0.3
+    keep = P.kept(n, p, 1, 0)
+    for bad in (np.inf, -np.inf, np.nan):
+        y = _got(jt.nn.dropout(jt.array(np.full(n, bad, np.float32)), p, True, seed=1))
+        assert (y[~keep] == 0).all() and (np.isnan(y[keep]) if np.isnan(bad) else y[keep] == bad).all()
+
+
+def test_dropout_of_nothing(gpu):
+    x = jt.array(np.zeros((0, 5), np.float32))
+    y = jt.nn.dropout(x, 0.5, True, seed=1)
+    assert y.numpy().shape == (0, 5) and jt.grad(y.sum(), x).numpy().shape == (0, 5)
+
+
+def test_dropout_replays_with_other_seeds(gpu):
+    """The same graph again and again: recorded launches take each call's seed, offset and buffers."""
+    rng = np.random.default_rng(3)
+    for turn in range(6):
+        x, xe = _make(rng, (37, 29), "float32")
+        h = x * 2.0
+        y = jt.nn.dropout(h, 0.25, True, seed=100 + turn, offset=turn << 33)
+        dx = jt.grad((y * y).sum(), x)
+        jt.sync([y, dx])
+        keep = P.kept(x.num, 0.25, 100 + turn, turn << 33).reshape(x.shape)
+        f = np.float64(np.float32(4.0 / 3.0))
+        _check(_got(y), np.where(keep, 2 * xe * f, 0.0), 4 * E * np.abs(xe), "float32", turn)
+        _check(_got(dx), np.where(keep, 8 * xe * f * f, 0.0), 64 * E * np.abs(xe), "float32", turn)
+
+
+def test_dropout_past_32_bits(gpu):
+    """Elements behind 2^32: the counter's upper word."""
+    n = (1 << 32) + 8 * 37
+    x = core.Var([n], "float16")
+    jt.sync([])
+    buf = core.Buffer(2 * n)
+    x._buf = buf
+    gpu.check(gpu.load().mjt_fill_u32(buf.ptr, 0x3C003C00, n // 2))
+    y = jt.nn.dropout(x, 0.5, True, seed=5, offset=1)
+    y.sync()
+    at = (1 << 32) - 64
+    tail = gpu.d2h(y._buf.ptr + 2 * at, [n - at], np.float16)
+    for k, v in enumerate(tail):
+        e = at + k
+        g = e // 8
+        b = P.philox([g & 0xFFFFFFFF, g >> 32, 1, 0], [5, 0])
+        assert v == (2.0 if (b[e % 8 // 2] >> 16 * (e % 2)) & 0xFFFF >= 0x8000 else 0.0), e
+
+
+# ---- norms of heads and rotation ------------------------------------------------------------------------------------
+def _table(rng, n, pairs):
+    t = rng.uniform(0, 6.28, (n, pairs))
+    t = np.stack([np.cos(t), np.sin(t)], -1).astype(np.float32)
+    return jt.array(t), t.astype(np.float64)
+
+
+def _laid(a, lead, first):
+    """[tokens, heads, dim] as the operator writes it"""
+    a = a.reshape(tuple(lead) + a.shape[1:])
+    return np.swapaxes(a, -3, -2) if first else a
+
+
+def _heads(dtype, lead, hq, hk, dim, pairs, paired, first, sections=None, scaled=True, scale_dtype=None, per_sequence=False, given=(True, True, True), seed=0, want=(True, True, True)):
+    rng = np.random.default_rng(seed)
+    tokens, S = int(np.prod(lead)), lead[-1]
+    x, xe = _make(rng, tuple(lead) + (hq + 2 * hk, dim), dtype, 1.5)
+    xe = xe.reshape(tokens, hq + 2 * hk, dim)
+    sq = sk = sqe = ske = table = positions = cos = sin = None
+    if scaled:
+        (sq, sqe), (sk, ske) = (_make(rng, (dim,), scale_dtype or dtype, 0.3, 1.0) for _ in range(2))
+    if pairs:
+        rows = 40
+        table, te = _table(rng, rows, pairs)
+        axes = len(sections) if sections else 1
+        at = rng.integers(0, rows, (axes, S if per_sequence else tokens)).astype(np.int32)
+        positions = jt.array(at.reshape(([axes] if sections else []) + ([S] if per_sequence else list(lead))))
+        whole = np.tile(at, (1, tokens // S)) if per_sequence and S else at
+        cos, sin = P.angles_of(te, whole, sections or [pairs], lead)
+    outs = jt.nn.qkv_norm_rope(x, hq, hk, sq, sk, table, positions, sections=sections, eps=1e-5, interleaved=paired, heads_first=first)
+    parts = {"q": (slice(0, hq), sqe), "k": (slice(hq, hq + hk), ske), "v": (slice(hq + hk, None), None)}
+    loss, gs = None, {}
+    for name, o, use in zip("qkv", outs, given):
+        if use:
+            g, ge = _make(rng, tuple(o.shape), dtype)
+            gs[name] = np.swapaxes(ge, -3, -2).reshape(tokens, -1, dim) if first else ge.reshape(tokens, -1, dim)
+            term = (o * g).sum()
+            loss = term if loss is None else loss + term
+    targets = [x] + ([sq, sk] if scaled else [])
+    grads = jt.grad(loss, targets) if loss is not None else []
+    jt.sync(list(outs) + [d for d, w in zip(grads, want) if w])
+    dx, sums = np.zeros_like(xe), {}
+    dxs = np.zeros_like(xe)
+    for name, o in zip("qkv", outs):
+        rows_, scale = parts[name]
+        part = xe[:, rows_]
+        if name == "v":
+            assert np.array_equal(_got(o), _laid(part, lead, first)), "v"
+            if name in gs:
+                dx[:, rows_] = gs[name]
+            continue
+        z = part / np.sqrt((part * part).mean(-1, keepdims=True) + 1e-5) * scale if scaled else part
+        size = P.pair_size(z, cos, paired)
+        # mean of squares, root and quotient: up to dim / 2 + 8 roundings; two more multiplications and the turn
+        _check(_got(o), _laid(P.head_norm(part, scale, cos, sin, 1e-5, paired), lead, first), _laid((dim / 2 + 16) * E * size, lead, first), dtype, name)
+        if name in gs:
+            dx[:, rows_], ds, dxs[:, rows_], dss = P.head_norm_grad(part, scale, cos, sin, 1e-5, paired, gs[name])
+            sums[name] = (ds, dss)
+    if loss is None:
+        return
+    if want[0]:
+        _check(_got(grads[0]).reshape(dx.shape), dx, (2 * dim + 32) * E * dxs, dtype, "dx")
+    if scaled:
+        for name, d, w in zip("qk", grads[1:], want[1:]):
+            if not w:
+                continue
+            ds, dss = sums.get(name, (np.zeros(dim), np.zeros(dim)))
+            _check(_got(d), ds, (tokens * (hq + 2 * hk) + dim + 32) * E * dss, scale_dtype or dtype, "d" + name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("paired", [False, True])
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("lead,hq,hk,dim,pairs", [((1, 1), 1, 1, 2, 1), ((2, 5), 4, 2, 128, 64), ((3, 7), 3, 1, 80, 40), ((1, 33), 5, 5, 64, 16), ((2, 9), 2, 1, 6, 2), ((1, 4), 2, 1, 258, 65)])
+def test_head_norms_and_rotation(gpu, dtype, paired, first, lead, hq, hk, dim, pairs):
+    _heads(dtype, lead, hq, hk, dim, pairs, paired, first)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("sections,pairs", [([8, 16, 16], 40), ([3, 0, 5], 8), ([1] * 8, 8), ([4], 4)])
+@pytest.mark.parametrize("per_sequence", [False, True])
+def test_positions_on_several_axes(gpu, dtype, sections, pairs, per_sequence):
+    for paired in (False, True):
+        _heads(dtype, (2, 11), 3, 2, 80, pairs, paired, True, sections=sections, per_sequence=per_sequence, seed=len(sections))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_tokens_and_heads(gpu, dtype):
+    _heads(dtype, (3, 700), 16, 4, 128, 64, False, True, seed=4)
+    _heads(dtype, (5000,), 1, 1, 64, 32, True, False, seed=5)
+    _heads(dtype, (2, 3), 70, 10, 96, 48, False, True, seed=6)
+
+
+def test_without_rotation_without_norm_and_with_scales_of_another_type(gpu):
+    _heads("bfloat16", (2, 6), 4, 2, 64, 0, False, False)
+    _heads("bfloat16", (2, 6), 4, 2, 64, 32, False, True, scaled=False)
+    _heads("float16", (2, 6), 4, 2, 72, 36, True, True, scale_dtype="float32")
+    _heads("float32", (2, 6), 4, 2, 72, 10, True, True, scale_dtype="bfloat16")
+
+
+@pytest.mark.parametrize("given", [(True, False, False), (False, True, False), (False, False, True), (True, False, True)])
+def test_gradients_of_some_of_the_results(gpu, given):
+    _heads("float32", (2, 6), 4, 2, 64, 32, False, True, given=given)
+    _heads("bfloat16", (2, 6), 4, 2, 64, 32, True, False, given=given, want=(False, True, False))
+    _heads("bfloat16", (2, 6), 4, 2, 64, 32, True, False, given=given, want=(True, False, False))
+
+
+def test_long_heads(gpu):
+    _heads("float32", (2, 3), 2, 1, 1022, 511, False, True)
+    _heads("bfloat16", (2, 3), 2, 1, 1024, 512, True, True)
+
+
+def test_heads_that_are_zero_or_not_finite(gpu):
+    """A head of zeros stays zero; an infinity or NaN stays in its own head."""
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((1, 6, 4, 64)).astype(np.float32)
+    x[0, 1, 0] = 0.0
+    x[0, 2, 1, 5] = np.nan
+    x[0, 3, 2, 7] = np.inf
+    s = jt.array(np.ones(64, np.float32))
+    t, _ = _table(rng, 6, 32)
+    q, k, v = jt.nn.qkv_norm_rope(jt.array(x), 2, 1, s, s, t)
+    good = x.copy()
+    good[~np.isfinite(good)] = 1.0
+    q1, k1, v1 = jt.nn.qkv_norm_rope(jt.array(good), 2, 1, s, s, t)
+    q, k, v, q1, k1, v1 = (_got(u) for u in (q, k, v, q1, k1, v1))
+    assert (q[0, 1, 0] == 0).all() and np.isnan(q[0, 2, 1]).all() and np.isnan(k[0, 3, 0]).any() and np.array_equal(v, x[:, :, 3:].astype(np.float64), equal_nan=True)
+    q[0, 2, 1] = q1[0, 2, 1]
+    k[0, 3, 0] = k1[0, 3, 0]
+    assert np.array_equal(q, q1) and np.array_equal(k, k1)
+
+
+def test_positions_outside_the_table_make_nan_of_what_they_turn(gpu):
+    rng = np.random.default_rng(9)
+    x, g = (jt.array(rng.standard_normal((1, 5, 3, 16)).astype(np.float32)) for _ in range(2))
+    s = jt.array(np.ones(16, np.float32))
+    t, _ = _table(rng, 10, 4)
+    at = np.array([[0, 10, -1, 9, 2 ** 31 - 1]], np.int32)
+    q, k, v = jt.nn.qkv_norm_rope(x, 1, 1, s, s, t, jt.array(at))
+    dx = jt.grad((q * g[:, :, :1]).sum(), x)
+    bad = (at[0] < 0) | (at[0] >= 10)
+    q, k, v, dx = _got(q), _got(k), _got(v), _got(dx)
+    for y in (q, k):
+        assert np.isnan(y[0, bad, :, :8]).all() and np.isfinite(y[0, bad, :, 8:]).all() and np.isfinite(y[0, ~bad]).all()
+    assert np.isfinite(v).all() and np.isfinite(dx[0, ~bad]).all() and np.isnan(dx[0, bad][:, 0]).all() and (dx[0, :, 1:] == 0).all()
+
+
+def test_positions_count_along_each_sequence_where_there_are_none(gpu):
+    rng = np.random.default_rng(10)
+    x = jt.array(rng.standard_normal((3, 7, 4, 8)).astype(np.float32))
+    s = jt.array(np.ones(8, np.float32))
+    t, _ = _table(rng, 9, 4)
+    for first in (False, True):
+        a = jt.nn.qkv_norm_rope(x, 2, 1, s, s, t, heads_first=first)
+        b = jt.nn.qkv_norm_rope(x, 2, 1, s, s, t, jt.array(np.arange(7, dtype=np.int32)), heads_first=first)
+        for u, w in zip(a, b):
+            assert np.array_equal(_got(u), _got(w))
+
+
+def test_no_tokens(gpu):
+    s = jt.array(np.ones(8, np.float32))
+    x = jt.array(np.zeros((2, 0, 4, 8), np.float32))
+    outs = jt.nn.qkv_norm_rope(x, 2, 1, s, s)
+    dx, ds = jt.grad(outs[0].sum() + outs[2].sum(), [x, s])
+    assert outs[0].numpy().shape == (2, 0, 2, 8) and dx.numpy().shape == (2, 0, 4, 8) and (ds.numpy() == 0).all()
+
+
+def test_heads_of_one_kind(gpu):
+    rng = np.random.default_rng(11)
+    x, xe = _make(rng, (2, 5, 3, 32), "bfloat16")
+    s, se = _make(rng, (32,), "bfloat16", 0.3, 1.0)
+    t, te = _table(rng, 5, 16)
+    y = jt.nn.head_norm_rope(x, s, t, eps=1e-5)
+    cos, sin = P.angles_of(te, np.tile(np.arange(5), 2)[None], [16], None)
+    want = P.head_norm(xe.reshape(10, 3, 32), se, cos, sin, 1e-5, False)
+    ds = jt.grad(y.sum(), s)
+    _check(_got(y).reshape(10, 3, 32), want, 64 * E * P.pair_size(np.abs(want), cos, False) + 64 * E, "bfloat16", "y")
+    _, dse, _, dss = P.head_norm_grad(xe.reshape(10, 3, 32), se, cos, sin, 1e-5, False, np.ones((10, 3, 32)))
+    _check(_got(ds), dse, 128 * E * dss, "bfloat16", "ds")
+
+
+def test_one_launch_for_three_results_and_replays(gpu):
+    rng = np.random.default_rng(12)
+    s = jt.array(np.ones(64, np.float32))
+    t, te = _table(rng, 6, 32)
+    cos, sin = P.angles_of(te, np.arange(6)[None], [32], None)
+    for turn in range(5):
+        x, xe = _make(rng, (1, 6, 4, 64), "float32")
+        before = dict(jt.executor_stats)
+        outs = jt.nn.qkv_norm_rope(x, 2, 1, s, s, t)
+        dx = jt.grad((outs[0] * outs[0]).sum() + outs[1].sum(), x)
+        jt.sync(list(outs) + [dx])
+        if turn == 0:
+            assert jt.executor_stats["launches"] - before["launches"] <= 4         # forward, the seeds' two groups, backward
+        for o, rows in zip(outs[:2], (slice(0, 2), slice(2, 3))):
+            want = P.head_norm(xe[0][:, rows], np.ones(64), cos, sin, 1e-6, False)
+            _check(_got(o)[0], want, 64 * E * P.pair_size(np.abs(want), cos, False), "float32", turn)
+        # a turn changes no length: sum q^2 = dim for every head whatever x, so dx of the queries is the eps's share alone
+        assert np.abs(_got(dx)[0][:, :2]).max() < 1e-3
+
+
+# ---- gated projections ------------------------------------------------------------------------------------------------
+def _gated(dtype, rows, k, f, act, lead=None, seed=0):
+    rng = np.random.default_rng(seed)
+    (x, xe), (w, we), (g, ge) = _make(rng, (rows, k), dtype), _make(rng, (2 * f, k), dtype, 1.5 / max(1, k) ** 0.5), _make(rng, (rows, f), dtype)
+    y = jt.nn.gated_linear(x, w, act)
+    want, off = P.gated(xe, we, act)
+    _check(_got(y), want, off, dtype, "y alone")
+    y = jt.nn.gated_linear(x, w, act)
+    dx, dw = jt.grad((y * g).sum(), [x, w])
+    jt.sync([y, dx, dw])
+    _check(_got(y), want, off, dtype, "y")
+    (dxe, dxo), (dwe, dwo) = P.gated_grad(xe, we, act, ge, dtype)
+    _check(_got(dx), dxe, dxo, dtype, "dx")
+    _check(_got(dw), dwe, dwo, dtype, "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
+@pytest.mark.parametrize("rows,k,f", [(1, 64, 16), (3, 40, 24), (17, 129, 33), (70, 256, 96)])
+def test_gated_projections(gpu, dtype, act, rows, k, f):
+    _gated(dtype, rows, k, f, act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,f", [(1, 1, 1), (1, 4096, 48), (2, 72, 1), (16, 512, 640), (33, 2048, 16), (64, 8, 8), (65, 320, 100), (128, 64, 64), (129, 192, 260), (300, 448, 520), (1, 1000, 333),
+                                      (260, 1024, 1030), (513, 128, 384)])
+def test_gated_sizes(gpu, dtype, rows, k, f):
+    _gated(dtype, rows, k, f, "silu", seed=rows + k)
+
+
+def test_gated_large_tiles(gpu):
+    _gated("bfloat16", 2100, 256, 4100, "gelu")
+    _gated("float16", 2048, 512, 4096, "silu")
+
+
+@pytest.mark.parametrize("act,ends", [("silu", (0.0, np.inf)), ("gelu", (0.0, np.inf)), ("relu", (0.0, np.inf)), ("sigmoid", (0.0, 1.0))])
+@pytest.mark.parametrize("rows", [1, 200])
+def test_gates_at_the_ends_of_the_range(gpu, act, ends, rows):
+    """Gates of both infinities, of the type's extremes and NaN: the activation's limits, and gradients without NaN where it is flat."""
+    values = np.array([-np.inf, np.inf, -3e38, 3e38, -200.0, 200.0, np.nan, 0.0], np.float32)
+    x = np.zeros((rows, 8), np.float32)
+    x[:, 0] = 1.0
+    w = np.zeros((16, 8), np.float32)
+    w[:8, 0] = values
+    w[8:, 0] = 1.0
+    x[:, 1:] = 0.0
+    y = jt.nn.gated_linear(jt.array(x[:, :1].copy()), jt.array(w[:, :1].copy()), act)
+    got = _got(y)
+    low, high = ends
+    assert (got[:, [0, 2]] == low).all() and (got[:, 1] == high).all() and np.isnan(got[:, 6]).all()
+    assert np.allclose(got[:, 3], 3e38 if high == np.inf else 1.0, rtol=1e-6) and np.allclose(got[:, 5], 200.0 if high == np.inf else 1.0) and np.abs(got[:, 4]).max() < 1e-30
+    v = jt.array(x[:, :1].copy())
+    dw = _got(jt.grad(jt.nn.gated_linear(v, jt.array(w[:, :1].copy()), act).sum(), jt.array(w[:, :1].copy())))
+    assert np.isfinite(dw).all()                      # (a weight that the result does not depend on)
+    wv = jt.array(w[:, :1].copy())
+    dw = _got(jt.grad(jt.nn.gated_linear(v, wv, act).sum(), wv))[:, 0]
+    slope = 1.0 if high == np.inf else 0.0
+    assert (dw[[0, 2, 4]] == 0).all() and (dw[[1, 3, 5]] == rows * slope).all()
+
+
+def test_gated_of_nothing(gpu):
+    for rows, k, f in ((0, 8, 4), (3, 8, 0), (3, 0, 4)):
+        x, w = jt.array(np.zeros((rows, k), np.float32)), jt.array(np.zeros((2 * f, k), np.float32))
+        y = jt.nn.gated_linear(x, w)
+        dx, dw = jt.grad(y.sum(), [x, w])
+        assert y.numpy().shape == (rows, f) and (y.numpy() == 0).all() and dx.numpy().shape == (rows, k) and dw.numpy().shape == (2 * f, k) and (dw.numpy() == 0).all()
+
+
+def test_gated_keeps_leading_axes_and_runs_the_forward_product_once(gpu):
+    rng = np.random.default_rng(5)
+    (x, xe), (w, we) = _make(rng, (2, 3, 40, 64), "bfloat16"), _make(rng, (64, 64), "bfloat16", 0.2)
+    y = jt.nn.gated_linear(x, w)
+    dx, dw = jt.grad(y.sum(), [x, w])
+    jt.sync([y, dx, dw])
+    want, off = P.gated(xe.reshape(-1, 64), we, "silu")
+    assert y.shape == [2, 3, 40, 32] and dx.shape == [2, 3, 40, 64]
+    _check(_got(y).reshape(-1, 32), want, off, "bfloat16", "y")
+    (dxe, dxo), (dwe, dwo) = P.gated_grad(xe.reshape(-1, 64), we, "silu", np.ones((240, 32)), "bfloat16")
+    _check(_got(dx).reshape(-1, 64), dxe, dxo, "bfloat16", "dx")
+    _check(_got(dw), dwe, dwo, "bfloat16", "dw")
+
+
+def test_gradients_asked_for_after_the_result_has_been_computed(gpu):
+    rng = np.random.default_rng(6)
+    (x, xe), (w, we) = _make(rng, (130, 64), "float16"), _make(rng, (192, 64), "float16", 0.2)
+    y = jt.nn.gated_linear(x, w, "gelu")
+    y.sync()
+    dx, dw = jt.grad((y * 2.0).sum(), [x, w])
+    (dxe, dxo), (dwe, dwo) = P.gated_grad(xe, we, "gelu", np.full((130, 96), 2.0), "float16")
+    _check(_got(dx), dxe, dxo, "float16", "dx")
+    _check(_got(dw), dwe, dwo, "float16", "dw")
+
+
+def test_gated_replays(gpu):
+    rng = np.random.default_rng(7)
+    w, we = _make(rng, (256, 128), "bfloat16", 0.1)
+    for turn in range(5):
+        x, xe = _make(rng, (40, 128), "bfloat16")
+        y = jt.nn.gated_linear(x, w)
+        dx, dw = jt.grad((y * 1.0).sum(), [x, w])
+        jt.sync([y, dx, dw])
+        want, off = P.gated(xe, we, "silu")
+        _check(_got(y), want, off, "bfloat16", turn)
+        (dxe, dxo), (dwe, dwo) = P.gated_grad(xe, we, "silu", np.ones((40, 128)), "bfloat16")
+        _check(_got(dx), dxe, dxo, "bfloat16", turn)
+        _check(_got(dw), dwe, dwo, "bfloat16", turn)
+
+
+@pytest.mark.parametrize("m,k,n,ta,tb", [(40, 30, 20, 0, 0), (256, 512, 256, 0, 1), (512, 256, 512, 1, 0), (64, 4096, 64, 1, 0), (7, 33, 9, 0, 1)])
+def test_products_rounded_to_nearest(gpu, m, k, n, ta, tb):
+    """mjt_matmul_nearest on each of the product kernels' routes: whole, in slices, plain."""
+    import ctypes
+    from jittor_amd import _lib as L
+    rng = np.random.default_rng(m)
+    (a, ae), (b, be) = _make(rng, (k, m) if ta else (m, k), "bfloat16"), _make(rng, (n, k) if tb else (k, n), "bfloat16")
+    c = core.Var([m, n], "bfloat16")
+    jt.sync([a, b])
+    c._buf = core.Buffer(c.nbytes)
+    t = [L.tensor(v._device_ptr(), v.dtype, v.shape) for v in (a, b, c)]
+    L.check(L.load().mjt_matmul_nearest(*[ctypes.byref(u) for u in t], ta, tb))
+    x, y = ae.T if ta else ae, be.T if tb else be
+    _check(bf16_bits_to_f32(L.d2h(c._buf.ptr, c.shape, np.uint16)).astype(np.float64), x @ y, (k + 2) * E * (np.abs(x) @ np.abs(y)), "bfloat16", "c")
