@@ -9,6 +9,7 @@ Nothing executes until a Var is synchronised (lazy_execution,
 var_holder.cc:25-33); execution is in executor.py.
 """
 import collections
+import ctypes
 import numbers
 import threading
 import weakref
@@ -721,6 +722,7 @@ _MAX_DIM = _lib.MAX_DIM
 
 # made natively (csrc/py/graph.cpp): a step builds hundreds of these
 _graph.setup(globals())
+_graph.set_launch(ctypes.cast(_lib.load().mjt_record_launch, ctypes.c_void_p).value)
 unary, binary, ternary, broadcast, reduce, make_number = _graph.unary, _graph.binary, _graph.ternary, _graph.broadcast, _graph.reduce, _graph.make_number
 _as_var, _broadcast_mask, _reduce_mask = _graph.as_var, _graph.broadcast_mask, _graph.reduce_mask
 

@@ -38,6 +38,16 @@
 // a[10]: bytes of x (the copies are range-checked by the dword).  Bound by the copies' latency at few tiles, else by memory: 64
 // images of 1024 x 14 x 14 -> 256 take 14.1 us (31 MB, 5 at the rate of a copy; 37.9 when the general convolution gathered x).
 //
+// KTAIL = 1: K is a multiple of 8 only.  The last stage's copies of an operand with k innermost leave out the 16-byte chunks behind
+// a row's end (an offset past the buffer reads as zero), and an operand with m or n innermost reads zero behind its last row anyway.
+//
+// GATED > 0: gated projections, y[m][f] = act(a g^T) * (a u^T) for B = [2 N][K] = g above u (both operands with k innermost).  A
+// tile's columns are TN / 2 columns f of both: a wave's B rows are those of g for its WT / 2 columns and then those of u for the
+// same ones, so that gate and up of a result lie in the same lane and place of two of its accumulators; the rest of the kernel
+// does not know.  On the way out gate and up go through LDS, so that a lane has VS adjacent columns of both.  p.a[2] y (GATED & 1), p.a[7] their products
+// in 32 bits, [M][2 N] (GATED & 2).  The operands' bytes for a tile are those of a plain product of 2 N columns, and neither product makes a trip to memory
+// on the way to y.
+//
 // The MFMAs are spelled out, like the LDS reads and the waits, so that the order below is the schedule; the
 // accumulators live in the accumulation registers, which nothing but these MFMAs touches inside the loop (the
 // compiler takes a spelled-out MFMA for finished the moment it is issued).
@@ -57,6 +67,12 @@ typedef unsigned mjt_u32x4v __attribute__((ext_vector_type(4)));
 #endif
 #ifndef IMG
 #define IMG 0
+#endif
+#ifndef GATED
+#define GATED 0
+#endif
+#ifndef KTAIL
+#define KTAIL 0
 #endif
 #define PIECES ((IMG + 7) / 8)  // 16-byte pieces of a plane
 #define TM TILE
@@ -118,9 +134,13 @@ struct Params { void* a[12 + EPI_WORDS]; };
 #endif
 extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu(1, WPE))) void ENTRY(Params p) {
     const int M = (int)(long long)p.a[3], N = (int)(long long)p.a[4], K = (int)(long long)p.a[5];
+#if GATED
+    const long long lda = (long long)p.a[6], ldb = lda;
+#else
     const long long lda = (long long)p.a[6], ldb = (long long)p.a[7], ldc = (long long)p.a[8];
+#endif
     const unsigned short* __restrict__ A = (const unsigned short*)p.a[0] + (long long)blockIdx.y * (long long)p.a[9];
-    const unsigned short* __restrict__ B = (const unsigned short*)p.a[1] + (IMG ? 0 : (long long)blockIdx.y * (long long)p.a[10]);
+    const unsigned short* __restrict__ B = (const unsigned short*)p.a[1] + (IMG || GATED ? 0 : (long long)blockIdx.y * (long long)p.a[10]);
     __shared__ __attribute__((aligned(16))) unsigned char lds[NBUF * STAGE_BYTES];
 
     // Tile order: panels of 4 tile rows, inside a panel column by column.  Workgroups go round-robin over the
@@ -128,7 +148,8 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
     // tiles and finds the operand rows and columns it shares in its own L2.  The next matrix of a batch starts one XCD
     // further on unless its tiles spread evenly, so that matrices of fewer than eight do over all of them (us, bfloat16 a b^T,
     // before / so: 64 x 128 x 128 x 64 12.4 / 7.2, 64 x 512 x 512 x 256 44.4 / 37.1, 32 x 256 x 256 x 512 a^T b^T 15.8 / 10.4).
-    const int tiles_m = (M + TM - 1) / TM, tiles_n = (N + TN - 1) / TN;
+    constexpr int CN = GATED ? TN / 2 : TN;                          // columns of C that a tile has
+    const int tiles_m = (M + TM - 1) / TM, tiles_n = (N + CN - 1) / CN;
     const int tiles = tiles_m * tiles_n;
     int L;
     {
@@ -145,11 +166,11 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
         tn = within / rows_here;
         tm = panel * 4 + within - tn * rows_here;
     }
-    const int m0 = tm * TM, n0 = tn * TN;
+    const int m0 = tm * TM, n0 = tn * CN;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1;
-    const int nstages = K / KS;
+    const int nstages = KTAIL ? (K + KS - 1) / KS : K / KS;
 
     // Copies.  A stage is 64 instructions of 1 KB (32 per operand); wave w issues number 8w .. 8w+7 of each operand.
     // An operand with k innermost is staged [256 rows][64 k]: lane i of instruction j fills row 8 j + i / 8, position
@@ -177,6 +198,10 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
 #if IMG
         const int gp = n0 / 8 + (int)piece, img = gp / PIECES;                  // the piece among all planes' pieces
         voff_b[q] = gp * 8 < N ? (unsigned)img * (unsigned)(ldb * 2) + (unsigned)krow * (IMG * 2) + (unsigned)(gp - img * PIECES) * 16 : 0x80000000u;
+#elif GATED
+        // (a wave copies rows of g or of u only: half of a wave's rows are WT / 2 = 8 CPW)
+        const int col = (wave >> 1) * (WT / 2) + q * 8 + (lane >> 3);
+        voff_b[q] = (unsigned)(col < last_b ? col : last_b) * (unsigned)(ldb * 2) + chunk * 16;
 #elif B_KCONT
         voff_b[q] = (unsigned)(row < last_b ? row : last_b) * (unsigned)(ldb * 2) + chunk * 16;
 #else
@@ -193,6 +218,9 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
 #if IMG
     const __amdgpu_buffer_rsrc_t b_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)B, 0, (int)(long long)p.a[10], 0x00020000);
     const int b_step = KS * IMG * 2;
+#elif GATED
+    const __amdgpu_buffer_rsrc_t b_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(B + ((wave & 1 ? (long long)N : 0) + n0) * ldb), 0, 0x7fffffff, 0x00020000);
+    const int b_step = KS * 2;
 #elif B_KCONT
     const __amdgpu_buffer_rsrc_t b_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)n0 * ldb), 0, 0x7fffffff, 0x00020000);
     const int b_step = KS * 2;
@@ -204,13 +232,20 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
     auto copy_one = [&](auto qc, int s, int slot) {
         constexpr int q = decltype(qc)::v;
         const int st = s < nstages ? s : nstages - 1;               // past the end: a stage nobody reads
+#if KTAIL
+        // instruction q's rows lie 8 q further on, so that the chunk at a lane's position alternates between two
+        const int chunk = (lane & 7) ^ (((q & 1) * 4 + (lane >> 4)) & 7);
+        const unsigned past = (q < CPW ? A_KCONT : B_KCONT) && st * KS + chunk * 8 >= K ? 0x80000000u : 0u;
+#else
+        const unsigned past = 0;
+#endif
         __attribute__((address_space(3))) unsigned char* dst =
             (__attribute__((address_space(3))) unsigned char*)&lds[0] + slot * STAGE_BYTES + wave * (CPW * 1024);
         // (an immediate offset would move the place in memory along with the place in LDS)
         if constexpr (q < CPW)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (__attribute__((address_space(3))) void*)(dst + q * 1024), 16, (int)voff_a[q], st * a_step, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(a_rsrc, (__attribute__((address_space(3))) void*)(dst + q * 1024), 16, (int)(voff_a[q] | past), st * a_step, 0, 0);
         else
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(b_rsrc, (__attribute__((address_space(3))) void*)(dst + TM * 128 + (q - CPW) * 1024), 16, (int)voff_b[q - CPW], st * b_step, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(b_rsrc, (__attribute__((address_space(3))) void*)(dst + TM * 128 + (q - CPW) * 1024), 16, (int)(voff_b[q - CPW] | past), st * b_step, 0, 0);
     };
     auto copy_stage = [&](int s, int slot) { mjt_static_for<0, 2 * CPW>([&](auto qc) { copy_one(qc, s, slot); }); };
 
@@ -330,6 +365,38 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
     mjt_static_for<0, NM>([&](auto ic) { mjt_pin(acc[decltype(ic)::v / FR][decltype(ic)::v % FR]); });
 
     // D of a 32x32 tile: lane holds column lane % 32, rows 8 * (e / 4) + 4 * (lane / 32) + e % 4.
+#if GATED
+    constexpr int WC = WT / 2, PITCH = WC + 8, LPR = WC / VS, IT = 32 * LPR / 64;                  // columns f of the wave; lanes a row; items a lane has of 32 rows
+    static_assert(4 * 2 * 32 * PITCH * 4 <= NBUF * STAGE_BYTES, "gate and up of a wave's 32 rows in LDS");
+    float* const mine = (float*)lds + wave * (2 * 32 * PITCH);
+    struct alignas(VS * 4) vec { float v[VS]; };
+#pragma unroll
+    for (int i = 0; i < FR; i++) {
+#pragma unroll
+        for (int j = 0; j < FR; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) mine[(j / (FR / 2) * 32 + 8 * (e / 4) + 4 * (lane >> 5) + (e & 3)) * PITCH + j % (FR / 2) * 32 + (lane & 31)] = acc[i][j][e];
+        mjt_wave_fence();
+#pragma unroll
+        for (int q = 0; q < IT; q++) {
+            const int lrow = (q * 64 + lane) / LPR, lcol = (q * 64 + lane) % LPR * VS, row = m0 + wm * WT + i * 32 + lrow, col = n0 + wn * WC + lcol;
+            if (row >= M || col >= N) continue;                                              // (VS divides N)
+            const vec gate = *(const vec*)&mine[lrow * PITCH + lcol], up = *(const vec*)&mine[(32 + lrow) * PITCH + lcol];
+            if constexpr (GATED & 2) {
+                float* both = (float*)p.a[7] + (long long)row * 2 * N + col;
+                *(vec*)both = gate;
+                *(vec*)(both + N) = up;
+            }
+            if constexpr (GATED & 1) {
+                struct alignas(VS * 2) { unsigned short v[VS]; } o;
+#pragma unroll
+                for (int k = 0; k < VS; k++) o.v[k] = mjt_el<IN>::down(mjt_activate(gate.v[k]).a * up.v[k]);
+                *(decltype(o)*)((unsigned short*)p.a[2] + (long long)row * N + col) = o;
+            }
+        }
+        mjt_wave_fence();                                                                // (before the next 32 rows overwrite these)
+    }
+#else
     const long long c0 = (long long)blockIdx.y * (long long)p.a[11];
 #if EPI || VS == 4
     // A wave's results go through LDS, 32 rows at a time, so that a lane has VS adjacent columns and an instruction whole 128-byte
@@ -428,5 +495,6 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
                 }
             }
         }
+#endif
 #endif
 }

@@ -1,5 +1,6 @@
 // mjt_gated_linear and the element-wise part of its gradient; mjt_matmul_nearest.
 #include "common.h"
+#include <cmath>
 
 namespace mjt {
 
@@ -34,6 +35,56 @@ void rows_pass(int act, const void* both, const void* y, const void* d, int dtyp
     jit_launch(k, (unsigned)std::min((n + 255) / 256, int64_t(1) << 23), 1, 256, 0, {bits_of_ptr(both), bits_of_ptr(y), bits_of_ptr(d), (uint64_t)n, (uint64_t)(F / V)});
 }
 
+bool forced(const char* route) {          // (a switch for measurements and tests: few, tiles or product)
+    const char* e = getenv("MJT_GATED");
+    return e && !strcmp(e, route);
+}
+
+// Up to 64 rows: one pass over the weights (kernels/gated_few.h).  False: not covered.
+bool few_rows(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
+    const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2, esz = dtype_size(x->dtype);
+    if (M > 64 || K == 0 || K * esz % 16 || K >= (int64_t(1) << 30) || F >= (int64_t(1) << 30) || (uintptr_t)x->ptr % 16 || (uintptr_t)w->ptr % 16 || (!forced("few") && getenv("MJT_GATED"))) return false;
+    const int MB = (int)((M + 15) / 16), RB = 1, W = 4, UN = 4;
+    std::ostringstream name, defs;
+    name << "mjt_gated_few_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << "_" << MB * 16 << (both ? y ? "_both" : "_products" : "");
+    defs << "#define TYPE " << element_type(x->dtype) << "\n#define ACT " << act << "\n#define W " << W << "\n#define RB " << RB << "\n#define MB " << MB << "\n#define UN " << UN << "\n#define BOTH "
+         << (both ? 1 : 0) << "\n#define Y " << (y ? 1 : 0) << "\n";
+    JitKernel* k = layer_kernel(name.str(), {"element.h", "gated_act.h", "gated_few.h"}, defs.str());
+    jit_launch(k, (unsigned)((F + 16 * RB - 1) / (16 * RB)), 1, W * 64, 0,
+               {bits_of_ptr(x->ptr), bits_of_ptr(w->ptr), bits_of_ptr(y ? y->ptr : nullptr), bits_of_ptr(both ? both->ptr : nullptr), (uint64_t)M, (uint64_t)F, (uint64_t)K});
+    return true;
+}
+
+// 16-bit operands: gate and up on the same tiles of the matrix product's kernel (kernels/gemm_dma.h with GATED).  False: not covered.
+bool on_tiles(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
+    Context& c = ctx();
+    const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2;
+    if (dtype_size(x->dtype) != 2 || K % 8 || K < 64 || K * 2 * 256 >= (int64_t(1) << 31) || M >= (int64_t(1) << 31) || F >= (int64_t(1) << 30) || (uintptr_t)x->ptr % 16 || (uintptr_t)w->ptr % 16 ||
+        (!forced("tiles") && getenv("MJT_GATED")))
+        return false;
+    const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
+    int tile = 0;
+    for (int t = 256; t >= 128 && !tile; t /= 2) {
+        const int64_t tm = (M + t - 1) / t, tn = (F + t / 2 - 1) / (t / 2);
+        const double edge = ((double)M * F) / ((double)tm * t * tn * (t / 2)), tiles = (double)tm * tn, util = tiles / (std::ceil(tiles / cus) * cus);
+        if (t == 128 || (edge >= 0.85 && util >= 0.7 && K >= 256)) tile = t;
+    }
+    const int64_t tm = (M + tile - 1) / tile, tn = (F + tile / 2 - 1) / (tile / 2);
+    const int nbuf = tile == 256 ? 2 : tm * tn > cus ? 2 : 4, wpe = tile == 128 && nbuf == 2 ? 2 : 1;
+    auto whole = [&](int v) { return F % v == 0 && (!y || (uintptr_t)y->ptr % (size_t)(v * 2) == 0) && (!both || (uintptr_t)both->ptr % (size_t)(v * 4) == 0); };
+    const int vs = whole(4) ? 4 : whole(2) ? 2 : 1, tail = K % 64 ? 1 : 0, gated = (y ? 1 : 0) + (both ? 2 : 0);
+    std::ostringstream name, defs;
+    name << "mjt_gated_tiles_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << "_" << tile << "x" << tile << (wpe == 2 ? "_direct2" : "_direct") << (tail ? "_tail" : "") << (both ? y ? "_both" : "_products" : "");
+    defs << "#define VS " << vs << "\n#define IN " << element_type(x->dtype) << "\n#define OUT 2\n#define A_KCONT 1\n#define B_KCONT 1\n#define TILE " << tile << "\n#define NBUF " << nbuf << "\n#define WPE " << wpe
+         << "\n#define GATED " << gated << "\n#define KTAIL " << tail << "\n#define ACT " << act << "\n";
+    JitKernel* k = layer_kernel(name.str(), {"element.h", "gated_act.h", "gemm_dma.h"}, defs.str());
+    // (as for the plain product: a build that moved registers aside behind the spelled-out reads is not run)
+    if (k->spilled != 0 || k->agprs < 0 || k->agprs > tile * tile / 256) return false;
+    jit_launch(k, (unsigned)((tm * tn + 7) / 8 * 8), 1, 256, 0,
+               {bits_of_ptr(x->ptr), bits_of_ptr(w->ptr), bits_of_ptr(y ? y->ptr : nullptr), (uint64_t)M, (uint64_t)F, (uint64_t)K, (uint64_t)K, bits_of_ptr(both ? both->ptr : nullptr), 0, 0, 0, 0});
+    return true;
+}
+
 void forward(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
     require_init();
     act_name(act);
@@ -53,7 +104,8 @@ void forward(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor
         MJT_CHECK(both->ndim == 2 && both->dtype == MJT_FLOAT32 && both->shape[0] == M && both->shape[1] == 2 * F, "gated_linear: gate and up are " << shape_str(both) << " or not float32");
     }
     if (M == 0 || F == 0) return;
-    // both projections as one product in 32 bits, then the activation
+    if (few_rows(x, w, act, y, both) || on_tiles(x, w, act, y, both)) return;
+    // the rest: both projections as one product in 32 bits, then the activation
     mjt_tensor c{};
     if (both) c = *both;
     else {

@@ -17,6 +17,7 @@
 #include <string>
 #include <unordered_map>
 #include <unordered_set>
+#include <memory>
 #include <vector>
 
 namespace {
@@ -37,7 +38,7 @@ struct Ref {
 PyObject* keep(PyObject* p) { Py_XINCREF(p); return p; }
 
 #define NAMES(X) X(shape) X(num) X(dtype) X(_op) X(_history) X(id) X(_out_ref) X(inputs) X(amp) X(op) X(bcast_mask) X(keepdims_mask) X(reduce_mask) X(is_scalar) \
-    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) X(call) X(index) \
+    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) X(call) X(index) X(ptr) X(_device_ptr) X(int64) X(int32) \
     X(_binary_dtypes) X(binary_dtype_infer) X(unary_dtype_infer) X(reduce_dtype_infer) X(dtype_infer) X(cast) X(add) X(mean) X(float16) X(bfloat16) X(float32)
 #define DECLARE(n) PyObject* s_##n;
 NAMES(DECLARE)
@@ -1093,6 +1094,218 @@ PyObject* py_signature(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return rest ? PyTuple_Pack(2, bytes.p, rest.p) : nullptr;
 }
 
+// ---- replays --------------------------------------------------------------------------------------------------------------------
+// A plan of the executor whose launches are recorded (executor.py: _Plan, _replay): gives the results of a graph their buffers and
+// issues the recording, as _replay does in byte code (us of host time a pass, there / here: one launch with three results 13.5 / 8.3, two with two 17.9 / 12.0).
+struct Plan {
+    struct Slot { int kind, op, input; bool needs; };          // kind 0: an input, 1: a result, 2: memory of its own for the replay
+    std::vector<Slot> slots;
+    std::vector<Ref> sizes;                                    // of kind 2
+    struct Made { int slot, from; };
+    std::vector<Made> made;
+    std::vector<Ref> made_sizes;
+    std::vector<int> scalars;                                  // their slots
+    std::vector<std::pair<int, bool>> cleared;
+    Ref buffer, scalar_value;
+};
+const char* const PLAN = "jittor_amd.plan";
+typedef int (*Launch)(void*, int, const uint64_t*, int, const double*, const int64_t*);
+Launch g_launch = nullptr;
+
+// plan(slots, needs_ptr, produce, scalars, cleared, Buffer, scalar_value)
+PyObject* py_plan(PyObject*, PyObject* args) {
+    PyObject *slots, *needs, *produce, *scalars, *cleared, *buffer, *scalar_value;
+    if (!PyArg_ParseTuple(args, "O!O!O!O!O!OO", &PyList_Type, &slots, &PySet_Type, &needs, &PyList_Type, &produce, &PyList_Type, &scalars, &PyList_Type, &cleared, &buffer, &scalar_value)) return nullptr;
+    std::unique_ptr<Plan> plan(new Plan);
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(slots); k++) {
+        PyObject* d = PyList_GET_ITEM(slots, k);
+        const char* kind;
+        int op = 0, input = 0;
+        Ref at(PyLong_FromSsize_t(k)), size;
+        if (!at || !PyTuple_Check(d) || PyTuple_GET_SIZE(d) < 2 || !(kind = PyUnicode_AsUTF8(PyTuple_GET_ITEM(d, 0)))) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_TypeError, "plan: a slot");
+        const int type = !strcmp(kind, "in") ? 0 : !strcmp(kind, "out") ? 1 : 2;
+        if (type == 2) size = Ref(keep(PyTuple_GET_ITEM(d, 1)));
+        else op = (int)PyLong_AsLong(PyTuple_GET_ITEM(d, 1));
+        if (type == 0) input = (int)PyLong_AsLong(PyTuple_GET_ITEM(d, 2));
+        const int has = PySet_Contains(needs, at.p);
+        if (has < 0 || PyErr_Occurred()) return nullptr;
+        plan->slots.push_back({type, op, input, has == 1});
+        plan->sizes.push_back(std::move(size));
+    }
+    const int n = (int)plan->slots.size();
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(produce); i++) {
+        int slot, from;
+        PyObject* size;
+        if (!PyArg_ParseTuple(PyList_GET_ITEM(produce, i), "iiO", &slot, &from, &size)) return nullptr;
+        if (slot < 0 || slot >= n || from >= n) return PyErr_Format(PyExc_IndexError, "plan: a slot");
+        plan->made.push_back({slot, from});
+        plan->made_sizes.push_back(Ref(keep(size)));
+    }
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(scalars); i++) {
+        PyObject *a, *b;
+        int slot;
+        if (!PyArg_ParseTuple(PyList_GET_ITEM(scalars, i), "OOi", &a, &b, &slot)) return nullptr;
+        if (slot < 0 || slot >= n) return PyErr_Format(PyExc_IndexError, "plan: a slot");
+        plan->scalars.push_back(slot);
+    }
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(cleared); i++) {
+        int op, inputs;
+        if (!PyArg_ParseTuple(PyList_GET_ITEM(cleared, i), "ip", &op, &inputs)) return nullptr;
+        plan->cleared.push_back({op, inputs != 0});
+    }
+    plan->buffer = Ref(keep(buffer));
+    plan->scalar_value = Ref(keep(scalar_value));
+    return PyCapsule_New(plan.release(), PLAN, [](PyObject* c) { delete (Plan*)PyCapsule_GetPointer(c, PLAN); });
+}
+
+// the address of mjt_record_launch
+PyObject* py_set_launch(PyObject*, PyObject* address) {
+    g_launch = (Launch)PyLong_AsVoidPtr(address);
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+}
+
+bool one_number(PyObject* v, PyObject* scalar_value, double* f, int64_t* i) {
+    PyObject *type = own(v, s_dtype), *host = own(v, s__host);
+    if (type && host && (type == s_int64 || type == s_int32)) {
+        Py_buffer view;
+        if (PyObject_GetBuffer(host, &view, PyBUF_SIMPLE) == 0) {
+            const bool wide = view.len == 8;
+            if (wide) memcpy(i, view.buf, 8);
+            else if (view.len == 4) {
+                int32_t narrow;
+                memcpy(&narrow, view.buf, 4);
+                *i = narrow;
+            }
+            const bool read = wide || view.len == 4;
+            PyBuffer_Release(&view);
+            *f = 0.0;
+            if (read) return true;
+        } else
+            PyErr_Clear();
+    }
+    Ref both(PyObject_CallOneArg(scalar_value, v));
+    if (!both) return false;
+    long long whole;
+    if (!PyArg_ParseTuple(both.p, "dL", f, &whole)) return false;
+    *i = whole;
+    return true;
+}
+
+// replay(plan, ops, recording): the library's status.  Where it is not 0 the results are as they were.
+PyObject* py_replay(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 3 || !PyList_Check(args[1]) || !g_launch) return PyErr_Format(PyExc_TypeError, "replay(plan, ops, recording)");
+    Plan* plan = (Plan*)PyCapsule_GetPointer(args[0], PLAN);
+    if (!plan) return nullptr;
+    PyObject* ops = args[1];
+    void* rec = PyLong_AsVoidPtr(args[2]);
+    if (!rec) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "replay: no recording");
+    const size_t n = plan->slots.size();
+    std::vector<Ref> var(n), buf(n);
+    std::vector<uint64_t> base(n, 0);
+    auto op_at = [&](int i) -> PyObject* {
+        if (i < 0 || i >= PyList_GET_SIZE(ops)) { PyErr_SetString(PyExc_IndexError, "replay: an op"); return nullptr; }
+        return PyList_GET_ITEM(ops, i);
+    };
+    auto address = [&](size_t k) {                             // of the buffer in buf[k]
+        PyObject* p = own(buf[k].p, s_ptr);
+        base[k] = p ? (uint64_t)PyLong_AsUnsignedLongLong(p) : 0;
+        if (!p) PyErr_SetString(PyExc_AttributeError, "a buffer without an address");
+        return p && !PyErr_Occurred();
+    };
+    auto result_of = [&](PyObject* op) -> PyObject* {          // borrowed
+        PyObject* ref = own(op, s__out_ref);
+        PyObject* out = ref && ref != Py_None ? PyWeakref_GetObject(ref) : nullptr;
+        if (!out || out == Py_None) { PyErr_SetString(PyExc_ReferenceError, "replay: a result that is gone"); return nullptr; }
+        return out;
+    };
+    auto fill = [&]() -> int {                                 // the library's status, or 1 with an exception set
+        for (size_t k = 0; k < n; k++) {
+            const Plan::Slot& d = plan->slots[k];
+            if (d.kind == 2) {
+                buf[k] = Ref(PyObject_CallOneArg(plan->buffer.p, plan->sizes[k].p));
+                if (!buf[k] || !address(k)) return 1;
+                continue;
+            }
+            PyObject* op = op_at(d.op);
+            if (!op) return 1;
+            if (d.kind == 1) {
+                PyObject* out = result_of(op);
+                if (!out) return 1;
+                var[k] = Ref(keep(out));
+                continue;
+            }
+            PyObject* ins = own(op, s_inputs);
+            if (!ins || !PyList_Check(ins) || d.input >= PyList_GET_SIZE(ins)) { PyErr_SetString(PyExc_IndexError, "replay: an input"); return 1; }
+            var[k] = Ref(keep(PyList_GET_ITEM(ins, d.input)));
+            if (!d.needs) continue;
+            if (absent(var[k].p, s__buf)) {                    // an array that is not on the device yet
+                Ref p(PyObject_CallMethodNoArgs(var[k].p, s__device_ptr));
+                if (!p) return 1;
+            }
+            PyObject* b = own(var[k].p, s__buf);
+            if (!b || b == Py_None) { PyErr_SetString(PyExc_RuntimeError, "replay: an input without a buffer"); return 1; }
+            buf[k] = Ref(keep(b));
+            if (!address(k)) return 1;
+        }
+        for (size_t i = 0; i < plan->made.size(); i++) {
+            const size_t k = (size_t)plan->made[i].slot;
+            PyObject* b = plan->made[i].from >= 0 ? buf[(size_t)plan->made[i].from].p : own(var[k].p, s__buf);
+            Ref fresh(b && b != Py_None ? keep(b) : PyObject_CallOneArg(plan->buffer.p, plan->made_sizes[i].p));
+            if (!fresh || PyDict_SetItem(dict_of(var[k].p), s__buf, fresh.p)) return 1;
+            buf[k] = std::move(fresh);
+            if (!address(k)) return 1;
+        }
+        std::vector<double> f(plan->scalars.size() + 1);
+        std::vector<int64_t> w(plan->scalars.size() + 1);
+        for (size_t i = 0; i < plan->scalars.size(); i++)
+            if (!one_number(var[(size_t)plan->scalars[i]].p, plan->scalar_value.p, &f[i], &w[i])) return 1;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = g_launch(rec, (int)n, base.data(), (int)plan->scalars.size(), f.data(), w.data());
+        Py_END_ALLOW_THREADS
+        return rc;
+    };
+    const int rc = fill();
+    if (rc) {                                                  // none is computed, and a buffer would say that it is
+        PyObject *et, *ev, *tb;
+        PyErr_Fetch(&et, &ev, &tb);
+        for (auto& m : plan->made) {
+            PyObject* v = var[(size_t)m.slot].p;
+            if (v && !absent(v, s__op) && PyDict_SetItem(dict_of(v), s__buf, Py_None)) PyErr_Clear();
+        }
+        PyErr_Restore(et, ev, tb);
+        return rc == 1 ? nullptr : PyLong_FromLong(rc);
+    }
+    for (auto& [i, inputs] : plan->cleared) {
+        PyObject* op = op_at(i);
+        PyObject* out = op ? result_of(op) : nullptr;
+        if (!out || PyDict_SetItem(dict_of(out), s__op, Py_None)) return nullptr;
+        if (inputs && !put(dict_of(op), s_inputs, PyList_New(0))) return nullptr;
+    }
+    return PyLong_FromLong(0);
+}
+
+// ---- results of library calls ------------------------------------------------------------------------------------------------------
+// kernel_var(KernelOp, call, index, inputs, shape, dtype): one result of a call (core.KernelOp), the list of its extents taken over
+PyObject* py_kernel_var(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 6 || !PyType_Check(args[0]) || !PyList_Check(args[3]) || !PyList_Check(args[4])) return PyErr_Format(PyExc_TypeError, "kernel_var(type, call, index, inputs, shape, dtype)");
+    const Py_ssize_t n = PyList_GET_SIZE(args[3]);
+    for (Py_ssize_t i = 0; i < n; i++)
+        if (!is_var(PyList_GET_ITEM(args[3], i))) return PyErr_Format(PyExc_TypeError, "kernel_var: inputs are Vars");
+    Shape s;
+    long long num;
+    if (!read_shape(args[4], &s)) return nullptr;
+    if (s.n < 1 || s.n > g_max_dim) return PyErr_Format(PyExc_ValueError, "at most %lld dims are supported", g_max_dim);
+    if (!count_elements(s, &num)) return nullptr;
+    PyObject* od;
+    std::vector<PyObject*> ins;
+    for (Py_ssize_t i = 0; i < n; i++) ins.push_back(PyList_GET_ITEM(args[3], i));
+    Ref op(new_op((PyTypeObject*)args[0], ins.data(), (int)n, &od));
+    if (!op || PyDict_SetItem(od, s_call, args[1]) || PyDict_SetItem(od, s_index, args[2])) return nullptr;
+    return new_var(keep(args[4]), args[5], op.p, num, false);
+}
+
 PyObject* py_as_var(PyObject*, PyObject* v) { return as_var(v); }
 
 PyObject* py_setup(PyObject*, PyObject* ns) {
@@ -1129,6 +1342,10 @@ PyMethodDef methods[] = {
     {"pending_ops", py_pending_ops, METH_O, "pending producers behind the targets, in topological order"},
     {"zero_number", py_zero_number, METH_O, "zero_number(var): whether it is one element in host memory whose bytes are all zero"},
     {"signature", (PyCFunction)(void (*)(void))py_signature, METH_FASTCALL, "signature(ops, targets, flags): hashable description of a graph, or None"},
+    {"plan", py_plan, METH_VARARGS, "plan(slots, needs_ptr, produce, scalars, cleared, Buffer, scalar_value): a plan for replay"},
+    {"replay", (PyCFunction)(void (*)(void))py_replay, METH_FASTCALL, "replay(plan, ops, recording): gives results their buffers and issues recorded launches; the library's status"},
+    {"set_launch", py_set_launch, METH_O, "takes the address of mjt_record_launch"},
+    {"kernel_var", (PyCFunction)(void (*)(void))py_kernel_var, METH_FASTCALL, "kernel_var(type, call, index, inputs, shape, dtype): a result of a library call"},
     {"gradients", (PyCFunction)(void (*)(void))py_gradients, METH_FASTCALL, "gradients(loss, targets, others): a gradient per target"},
     {"setup", py_setup, METH_O, "takes the classes and tables of core.py"},
     {nullptr, nullptr, 0, nullptr}};

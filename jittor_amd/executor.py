@@ -491,8 +491,9 @@ class _Recording:
 
 
 class _Plan:
-    # native: None until the plan has been replayed by its calls, then its _Recording, or False where the calls cannot be recorded
-    __slots__ = ("slots", "needs_ptr", "produce", "ptrs", "scalars", "calls", "stats", "cleared", "seen", "native")
+    # native: None until the plan has been replayed by its calls, then its _Recording, or False where the calls cannot be recorded;
+    # placed: the plan's slots as _graph.replay reads them, made with the recording
+    __slots__ = ("slots", "needs_ptr", "produce", "ptrs", "scalars", "calls", "stats", "cleared", "seen", "native", "placed")
 
 
 _cap = None
@@ -579,7 +580,7 @@ def _capture(ops, target_ids, sig):
             produce.append((k, src, 0))
             needs_ptr.add(src)
     plan.slots, plan.needs_ptr, plan.produce, plan.calls = slots, needs_ptr, produce, cap.calls
-    plan.seen, plan.native = 0, None
+    plan.seen, plan.native, plan.placed = 0, None, None
     plan.stats = [(key, stats[key] - before[key]) for key in stats if stats[key] != before[key]]
     plan.cleared = [(i, had_inputs[i] and not op.inputs) for i, op in enumerate(ops) if op.out is not None and op.out._op is None]
     if len(_plans) >= _PLAN_LIMIT:
@@ -637,15 +638,17 @@ def _record(plan):
             lib.mjt_record_free(rec)
 
 
-def _launch(plan, base, scalars):
+def _launch(plan, base, scalars, record=True):
     """The plan's calls on these buffers and scalars.  The calls look their kernels up and lay out parameters anew each time
     (3 us a call); from the third execution of a graph on the launches themselves are issued, all by one call."""
-    if plan.native is None:
+    if plan.native is None and record:
         if plan.seen:
             plan.native = _record(plan)
+            if plan.native:
+                plan.placed = _graph.plan(plan.slots, plan.needs_ptr, plan.produce, plan.scalars, plan.cleared, Buffer, _scalar_value)
         plan.seen += 1
     r = plan.native
-    if r:
+    if r:                                                      # (made just now: the next time _replay issues it)
         rc = _lib.load().mjt_record_launch(r.rec, r.n, r.bases(*base), r.ns, r.fvalues(*[f for f, _ in scalars]),
                                            r.ivalues(*[i for _, i in scalars]))
         if rc == 0:
@@ -653,7 +656,7 @@ def _launch(plan, base, scalars):
             return
         if rc != _lib.ERR_UNSUPPORTED:
             _lib.check(rc)
-        plan.native = None                                     # out of date (scratch memory of the library has moved): made again next time
+        plan.native = None                                     # out of date already: made again next time
     _fill_in(plan, base, scalars)
     check = _lib.check
     for fn, args in plan.calls:
@@ -663,6 +666,18 @@ def _launch(plan, base, scalars):
 
 
 def _replay(plan, ops):
+    record = True
+    if plan.native:
+        rc = _graph.replay(plan.placed, ops, plan.native.rec.value)
+        if rc == 0:
+            stats["recorded_launches"] += 1
+            for key, d in plan.stats:
+                stats[key] += d
+            stats["replays"] += 1
+            return
+        if rc != _lib.ERR_UNSUPPORTED:
+            _lib.check(rc)
+        plan.native, record = None, False                      # out of date (scratch memory of the library has moved): made again next time
     slots = plan.slots
     n = len(slots)
     var, buf, base = [None] * n, [None] * n, [0] * n
@@ -687,7 +702,7 @@ def _replay(plan, ops):
                 b = Buffer(nbytes)
             v._buf = buf[k] = b
             base[k] = b.ptr
-        _launch(plan, base, [_scalar_value(var[k]) for _, _, k in plan.scalars])
+        _launch(plan, base, [_scalar_value(var[k]) for _, _, k in plan.scalars], record)
     except BaseException:
         for k, _, _ in plan.produce:                           # none is computed, and a buffer would say that it is
             if var[k]._op is not None:

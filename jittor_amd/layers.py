@@ -9,6 +9,7 @@ import numbers
 
 import numpy as np
 
+from . import _graph
 from . import _lib
 from . import core
 from .core import KernelOp, Var
@@ -28,7 +29,7 @@ class Call:
 
 
 def _result(call, index, inputs, shape, dtype):
-    return Var(shape, dtype, KernelOp(list(inputs), call, index))
+    return _graph.kernel_var(KernelOp, call, index, inputs, shape, dtype)
 
 
 def _float_var(who, v, name="x"):
@@ -60,8 +61,10 @@ def _number(value, name):
     """64 bits that go into the kernel by value."""
     if not isinstance(value, numbers.Integral):
         raise TypeError("dropout: %s has to be an integer, got %r" % (name, value))
-    value = int(value) & (1 << 64) - 1
-    return core.from_storage(np.array([value], np.uint64).view(np.int64), "int64")
+    v = Var([1], "int64", None, 1)
+    v._host = np.array([int(value) & (1 << 64) - 1], np.uint64).view(np.int64)
+    v.is_scalar = True
+    return v
 
 
 def dropout(x, p, is_train, seed, offset, residual):
@@ -234,7 +237,7 @@ def _gated_gradients(op, inputs, douts, wanted):
     dy = douts[0]
     f2 = w.shape[0]
     # the products of the forward pass in 32 bits: written by the same launch where the two passes run together, made again otherwise
-    both = _result(op.call, 1, inputs, list(x.shape[:-1]) + [f2], "float32")
+    both = _result(op.call, 1, list(inputs), list(x.shape[:-1]) + [f2], "float32")
     d = _result(Call("gated_linear_grad", *op.call.options), 0, [dy, both], list(x.shape[:-1]) + [f2], dy.dtype)
     return [_result(Call("product", False, False), 0, [d, w], list(x.shape), x.dtype) if wanted[0] else None,
             _result(Call("product", True, False), 0, [d, x], list(w.shape), w.dtype) if wanted[1] else None]
