@@ -209,6 +209,10 @@ struct Nearest {
     static bool on();
 };
 
+// Gated projections on the tiles of the general product kernel (op_matmul.cpp, kernels/gemm_mfma.h with GATED): rows of x and of the
+// weights [2 F, K] are whole 16-byte pieces that begin at one.  False, with nothing launched: the product is better cut into slices of its sum.
+bool gemm_gated(int dtype, int act, const char* act_name, const void* x, const void* w, void* y, void* both, int64_t M, int64_t F, int64_t K);
+
 // ---- operators of transformer layers (op_layers.cpp) ----
 // The number of a float type inside kernels/element.h, -1 for other types.
 int element_type(int dtype);

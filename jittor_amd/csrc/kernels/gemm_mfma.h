@@ -57,6 +57,10 @@
 // results are added up by a reduce launch.  Before, the shifted planes were written to memory, multiplied image by image
 // and the images' results added (float32 32 x 3 x 224 x 224, 7x7 stride 2 -> 64: 110 + 337 + 9 us; 116 here).
 //
+// GATED > 0: gated projections, y[m][f] = act(a g^T) * (a u^T) for B = [2 N][K] = g above u.  The tile's columns are TN / 2 columns f of g and the
+// same ones of u; its results go through LDS, where the two meet.  a[2] y (GATED & 1), a[7] their products in 32 bits, [M][2 N] (GATED & 2).  VS: adjacent columns
+// that a lane takes (4 or 1).
+//
 // Rows of A' and columns of B' beyond M and N are read from the last valid row (their
 // results are not stored); k beyond K is zeroed in both operands.  Leading dimensions are
 // multiples of 16 bytes and the operand pointers 16-byte aligned (the host sends
@@ -92,6 +96,9 @@ typedef unsigned short TIN;
 #define FJ (TN / 32 / WN)
 #ifndef CONV
 #define CONV 0
+#endif
+#ifndef GATED
+#define GATED 0
 #endif
 #ifndef SLICED
 #define SLICED 0                 // 1: workgroup (tile, slice) sums stages slice * a[9] .. of K into its own float32 C (or y), a[11] apart
@@ -206,7 +213,7 @@ template <int I, int N, class F> __device__ __forceinline__ void mjt_static_for(
 // A tile moves in PER pieces, one 16-byte move per thread each.  fetch() only issues piece I's load (unconditional: nothing in it
 // looks at a loaded value, so no wait is needed before the MFMAs that follow); commit() zeroes what lies beyond K, transposes
 // and writes to LDS.  FULL: the stage does not reach beyond K.
-template <int ROWS, bool KCONT> struct mjt_stager {
+template <int ROWS, bool KCONT, bool HALVES = false> struct mjt_stager {       // HALVES: the tile's rows are ROWS / 2 of rmax rows and the same of the rmax rows behind them
     static constexpr int PER = ROWS * KC / NTHR;          // 16-byte moves per thread
     mjt_u32x4v reg[PER];
 
@@ -214,8 +221,9 @@ template <int ROWS, bool KCONT> struct mjt_stager {
         if constexpr (KCONT) {
             // chunk c = tid + I * NTHR: row c / KC, k-chunk c % KC (8 consecutive lanes read one 128-byte line)
             const int c = tid + I * NTHR;
-            int row = r0 + c / KC;
+            int row = r0 + (HALVES ? c / KC % (ROWS / 2) : c / KC);
             row = row < rmax ? row : rmax - 1;
+            if (HALVES && c / KC >= ROWS / 2) row += rmax;
             const int k = k0 + (c % KC) * EPC;
             const int kk = FULL || k < K ? k : 0;         // a chunk past the end reads chunk 0 and is zeroed in commit
             reg[I] = *(const mjt_u32x4v*)(p + (long long)row * ld + kk);
@@ -470,7 +478,11 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
 #else
     const int K = (int)(long long)p.a[5];
 #endif
+#if GATED
+    const long long lda = (long long)p.a[6], ldb = lda;
+#else
     const long long lda = (long long)p.a[6], ldb = (long long)p.a[7], ldc = (long long)p.a[8];
+#endif
 #if CONV == 2
     const TIN* __restrict__ A = (const TIN*)p.a[0];
     const TIN* __restrict__ B = (const TIN*)p.a[1];
@@ -485,7 +497,8 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
     // grid to itself, rounded up to eight workgroups, and which compute units the empty ones kept from work was chance: float32
     // 64 x 256 x 196 x 1024 on 128 x 128 tiles, four a matrix, 92 / 56; 256 x 64 x 64 x 64 9.2 / 5.2; bfloat16 the same 7.1 / 4.0,
     // 100 x 200 x 200 x 128 22.2 / 12.2.)
-    const int tiles_m = (M + TM - 1) / TM, tiles_n = (N + TN - 1) / TN, tiles = tiles_m * tiles_n;
+    constexpr int CN = GATED ? TN / 2 : TN;                     // columns of the result that a tile has
+    const int tiles_m = (M + TM - 1) / TM, tiles_n = (N + CN - 1) / CN, tiles = tiles_m * tiles_n;
 #if CONV == 2 || SLICED
     const int per_slice = (int)(long long)p.a[9], pairs = ((K + KS - 1) / KS + per_slice - 1) / per_slice * tiles;
 #else
@@ -524,7 +537,7 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
         tn = within / rows_here;
         tm = panel * 4 + within - tn * rows_here;
     }
-    const int m0 = tm * TM, n0 = tn * TN;
+    const int m0 = tm * TM, n0 = tn * CN;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave / WN, wn = wave % WN;
 
@@ -580,7 +593,7 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
     const __amdgpu_buffer_rsrc_t x_rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)img0 * (C_ * H_) * W_), 0,
                                                                             (int)(x_bytes < 0x7fffffffll ? x_bytes : 0x7fffffffll), 0x00020000);
 #else
-    mjt_stager<TN, B_KCONT> sb[NSET];
+    mjt_stager<TN, B_KCONT, GATED != 0> sb[NSET];
 #endif
     constexpr int PA = TM * KC / NTHR, PIECES = PA + TN * KC / NTHR;
     auto fetch = [&](auto ic, auto setc, auto fullc, int stage) {
@@ -734,6 +747,38 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
     }
 #endif
 
+#if GATED
+    constexpr int PITCH = TN + 4, ITEMS = TM * CN / VS;
+    static_assert(TM * PITCH * 4 <= (int)sizeof(lds), "a tile's results in LDS");
+    float* const tile = (float*)&lds[0][0];
+    __syncthreads();                                           // every wave has read its last fragments
+#pragma unroll
+    for (int i = 0; i < FI; i++)
+#pragma unroll
+        for (int j = 0; j < FJ; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) tile[(wm * 32 * FI + i * 32 + 8 * (e / 4) + 4 * (lane >> 5) + (e & 3)) * PITCH + wn * 32 * FJ + j * 32 + (lane & 31)] = acc[i][j][e];
+    __syncthreads();
+    struct alignas(VS * 4) vec { float v[VS]; };
+#pragma unroll 4
+    for (int item = tid; item < ITEMS; item += NTHR) {
+        const int lrow = item / (CN / VS), lcol = item % (CN / VS) * VS, row = m0 + lrow, col = n0 + lcol;
+        if (row >= M || col >= N) continue;                    // (VS divides N)
+        const vec gate = *(const vec*)&tile[lrow * PITCH + lcol], up = *(const vec*)&tile[lrow * PITCH + CN + lcol];
+        if constexpr (GATED & 2) {
+            float* both = (float*)p.a[7] + (long long)row * 2 * N + col;
+            *(vec*)both = gate;
+            *(vec*)(both + N) = up;
+        }
+        if constexpr (GATED & 1) {
+            mjt_els<IN, VS> o;
+#pragma unroll
+            for (int k = 0; k < VS; k++) o.v[k] = mjt_el<IN>::down(mjt_activate(gate.v[k]).a * up.v[k]);
+            *(mjt_els<IN, VS>*)((typename mjt_el<IN>::raw*)p.a[2] + (long long)row * N + col) = o;
+        }
+    }
+    return true;
+#else
     // D of a 32x32 tile: lane holds column lane % 32, rows 8 * (e / 4) + 4 * (lane / 32) + e % 4
     const long long c0 = (long long)outer * (long long)p.a[11];
 #pragma unroll
@@ -780,6 +825,7 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
             }
         }
     return true;
+#endif
     };
 #if SPLIT
     if (multiply(mjt_ic<1>())) return;

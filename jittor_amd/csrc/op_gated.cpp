@@ -35,40 +35,54 @@ void rows_pass(int act, const void* both, const void* y, const void* d, int dtyp
     jit_launch(k, (unsigned)std::min((n + 255) / 256, int64_t(1) << 23), 1, 256, 0, {bits_of_ptr(both), bits_of_ptr(y), bits_of_ptr(d), (uint64_t)n, (uint64_t)(F / V)});
 }
 
-bool forced(const char* route) {          // (a switch for measurements and tests: few, tiles or product)
-    const char* e = getenv("MJT_GATED");
-    return e && !strcmp(e, route);
-}
-
-// Up to 64 rows: one pass over the weights (kernels/gated_few.h).  False: not covered.
-bool few_rows(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
-    const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2, esz = dtype_size(x->dtype);
-    if (M > 64 || K == 0 || K * esz % 16 || K >= (int64_t(1) << 30) || F >= (int64_t(1) << 30) || (uintptr_t)x->ptr % 16 || (uintptr_t)w->ptr % 16 || (!forced("few") && getenv("MJT_GATED"))) return false;
-    const int MB = (int)((M + 15) / 16), RB = 1, W = 4, UN = 4;
-    std::ostringstream name, defs;
-    name << "mjt_gated_few_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << "_" << MB * 16 << (both ? y ? "_both" : "_products" : "");
-    defs << "#define TYPE " << element_type(x->dtype) << "\n#define ACT " << act << "\n#define W " << W << "\n#define RB " << RB << "\n#define MB " << MB << "\n#define UN " << UN << "\n#define BOTH "
-         << (both ? 1 : 0) << "\n#define Y " << (y ? 1 : 0) << "\n";
-    JitKernel* k = layer_kernel(name.str(), {"element.h", "gated_act.h", "gated_few.h"}, defs.str());
-    jit_launch(k, (unsigned)((F + 16 * RB - 1) / (16 * RB)), 1, W * 64, 0,
-               {bits_of_ptr(x->ptr), bits_of_ptr(w->ptr), bits_of_ptr(y ? y->ptr : nullptr), bits_of_ptr(both ? both->ptr : nullptr), (uint64_t)M, (uint64_t)F, (uint64_t)K});
-    return true;
-}
-
-// 16-bit operands: gate and up on the same tiles of the matrix product's kernel (kernels/gemm_dma.h with GATED).  False: not covered.
-bool on_tiles(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
-    Context& c = ctx();
-    const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2;
-    if (dtype_size(x->dtype) != 2 || K % 8 || K < 64 || K * 2 * 256 >= (int64_t(1) << 31) || M >= (int64_t(1) << 31) || F >= (int64_t(1) << 30) || (uintptr_t)x->ptr % 16 || (uintptr_t)w->ptr % 16 ||
-        (!forced("tiles") && getenv("MJT_GATED")))
-        return false;
-    const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
-    int tile = 0;
-    for (int t = 256; t >= 128 && !tile; t /= 2) {
-        const int64_t tm = (M + t - 1) / t, tn = (F + t / 2 - 1) / (t / 2);
-        const double edge = ((double)M * F) / ((double)tm * t * tn * (t / 2)), tiles = (double)tm * tn, util = tiles / (std::ceil(tiles / cus) * cus);
-        if (t == 128 || (edge >= 0.85 && util >= 0.7 && K >= 256)) tile = t;
+// The ways to run the projections, by estimated time.
+//   FEW (kernels/gated_few.h): up to 16 rows.  16-bit operands of more than 4 rows and 24 MB of weights are better off on tiles, which load x once
+//   for 32 columns (us few / MFMA: 16 x 1024 -> 2816 6.4 / 7.4; 16 x 2048 -> 5632 14.7 / 10.8, of 4 rows 11.9 / 11.1); float32 MFMAs are slower
+//   than the loads of x (float32 16 x 2048 -> 5632 28 / 33).
+//   TILES (kernels/gemm_dma.h): 16-bit operands on 256 x 256 tiles, one to a compute unit, or 128 x 128, two to a unit.
+//   MFMA (kernels/gemm_mfma.h): any type; a product that is better cut into slices of its sum goes to PRODUCT, the plain product in 32 bits and a pass over it.
+// A stage of 64 elements of the sum takes 1.1 us on a 256 x 256 tile, 0.33 on a 128 x 128 tile with a unit to itself and 0.66 for two of them (more
+// where the sum is long and neighbours drift apart), 0.25 on a 64 x 64 tile; a round begins with the first loads and ends with the
+// activations and stores, 10, 6 and 3.5 us.  Rows that are no whole 128-byte lines cost a quarter more.
+// us measured 256 / 128 / MFMA for bfloat16: 64 x 2048 -> 5632 43 / 16.3 / 11.3; 256 x 2048 -> 5632 45 / 17.5 / 22.4; 1024 x 2048 -> 5632 49.7 / 54.5 / 54.4; 2048 x
+// 2048 -> 5632 103.6 / 92.4 / 106; 8192 x 2048 -> 5632 335 / 367 / 393; 512 x 4096 -> 11264 107 / 134 / 106; 777 x 1000 -> 2600 34.5 / 22.8 / 25.8; 512 x 1024 -> 2816
+// 28.5 / 11.5 / 13.9; 4096 x 512 -> 1376 23.0 / 20.2 / 24.1.
+enum Route { FEW, TILES, MFMA, PRODUCT };
+Route choose(int dtype, int64_t M, int64_t F, int64_t K, bool aligned, int* tile) {
+    const int64_t esz = dtype_size(dtype), cus = ctx().dry_run || ctx().prop.multiProcessorCount <= 0 ? 256 : ctx().prop.multiProcessorCount;
+    const char* forced = getenv("MJT_GATED");                  // (a switch for measurements and tests; a route that does not cover the call is left out all the same)
+    auto may = [&](const char* name) { return !forced || !strcmp(forced, name); };
+    if (!aligned || K == 0) return PRODUCT;
+    const double stages = std::ceil((double)K / 64.0);
+    auto rounds = [&](double tiles, double at_once) { return std::ceil(tiles / at_once); };
+    auto tiles_of = [&](int64_t rows, int64_t cols) { return (double)((M + rows - 1) / rows) * (double)((F + cols - 1) / cols); };
+    if (may("few") && M <= 16 && (forced || esz == 4 || M <= 4 || 2 * F * K * esz <= int64_t(24) << 20)) return FEW;
+    if (may("tiles") && esz == 2 && K >= 64 && K * 2 * 256 < (int64_t(1) << 31)) {
+        const double r256 = rounds(tiles_of(256, 128), (double)cus), n128 = tiles_of(128, 64);
+        const double t256 = r256 * (10.0 + 1.1 * stages) * (r256 > 1 ? 1.2 : 1.0);
+        const double t128 = n128 <= (double)cus ? 5.3 + 0.335 * stages : rounds(n128, 2.0 * (double)cus) * (6.0 + 0.66 * stages * (1.0 + std::max(0.0, stages - 32.0) / 64.0));
+        const double mfma = 3.5 + 0.25 * stages * (1.0 + 0.8 * (rounds(tiles_of(64, 32), (double)cus) - 1.0));
+        *tile = t256 < t128 ? 256 : 128;
+        if (const char* e = getenv("MJT_GEMM_DMA")) *tile = atoi(e) == 128 ? 128 : 256;
+        if (forced || std::min(t256, t128) < mfma) return TILES;
     }
+    return may("mfma") ? MFMA : PRODUCT;
+}
+
+void few_rows(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
+    const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2;
+    const int W = 8, UN = 2;
+    std::ostringstream name, defs;
+    name << "mjt_gated_few_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << (both ? y ? "_both" : "_products" : "");
+    defs << "#define TYPE " << element_type(x->dtype) << "\n#define ACT " << act << "\n#define W " << W << "\n#define UN " << UN << "\n#define BOTH " << (both ? 1 : 0) << "\n#define Y " << (y ? 1 : 0) << "\n";
+    JitKernel* k = layer_kernel(name.str(), {"element.h", "gated_act.h", "gated_few.h"}, defs.str());
+    jit_launch(k, (unsigned)((F + 7) / 8), 1, W * 64, 0,
+               {bits_of_ptr(x->ptr), bits_of_ptr(w->ptr), bits_of_ptr(y ? y->ptr : nullptr), bits_of_ptr(both ? both->ptr : nullptr), (uint64_t)M, (uint64_t)F, (uint64_t)K});
+}
+
+// False: the compiler made no build of it that can be run.
+bool on_tiles(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both, int tile) {
+    const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2, cus = ctx().dry_run || ctx().prop.multiProcessorCount <= 0 ? 256 : ctx().prop.multiProcessorCount;
     const int64_t tm = (M + tile - 1) / tile, tn = (F + tile / 2 - 1) / (tile / 2);
     const int nbuf = tile == 256 ? 2 : tm * tn > cus ? 2 : 4, wpe = tile == 128 && nbuf == 2 ? 2 : 1;
     auto whole = [&](int v) { return F % v == 0 && (!y || (uintptr_t)y->ptr % (size_t)(v * 2) == 0) && (!both || (uintptr_t)both->ptr % (size_t)(v * 4) == 0); };
@@ -104,7 +118,16 @@ void forward(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor
         MJT_CHECK(both->ndim == 2 && both->dtype == MJT_FLOAT32 && both->shape[0] == M && both->shape[1] == 2 * F, "gated_linear: gate and up are " << shape_str(both) << " or not float32");
     }
     if (M == 0 || F == 0) return;
-    if (few_rows(x, w, act, y, both) || on_tiles(x, w, act, y, both)) return;
+    const int64_t K = x->shape[1];
+    MJT_CHECK(M < (int64_t(1) << 31) && F < (int64_t(1) << 26) && K < (int64_t(1) << 30), "gated_linear: x " << shape_str(x) << " and weights " << shape_str(w) << " are too large");
+    int tile = 0;
+    const Route route = choose(x->dtype, M, F, K, K * dtype_size(x->dtype) % 16 == 0 && (uintptr_t)x->ptr % 16 == 0 && (uintptr_t)w->ptr % 16 == 0, &tile);
+    if (route == FEW) {
+        few_rows(x, w, act, y, both);
+        return;
+    }
+    if (route == TILES && on_tiles(x, w, act, y, both, tile)) return;
+    if (route != PRODUCT && gemm_gated(x->dtype, act, act_name(act), x->ptr, w->ptr, y ? y->ptr : nullptr, both ? both->ptr : nullptr, M, F, K)) return;
     // the rest: both projections as one product in 32 bits, then the activation
     mjt_tensor c{};
     if (both) c = *both;

@@ -75,6 +75,75 @@ Nearest::Nearest() { t_nearest++; }
 Nearest::~Nearest() { t_nearest--; }
 bool Nearest::on() { return t_nearest > 0; }
 
+// How the general kernel cuts a product: tiles of 64 mi x 64 ni, slices of the sum of `per` stages each, operands in bfloat16 parts or not.
+struct TileChoice {
+    int mi, ni;
+    int64_t slices, per, stages;
+    bool split;
+};
+static TileChoice choose_tiles(int in_dtype, int64_t M, int64_t N, int64_t K, int64_t batch, bool a_kcont, bool b_kcont, int tile_m, int tile_n, int64_t ldc) {
+    Context& c = ctx();
+    const int esz = dtype_size(in_dtype);
+    // Tile: the largest of 64 MI x 64 NI (MI, NI in 1, 2, 4) that still gives every compute unit work and wastes
+    // little on the edges; larger tiles read each operand element less often.
+    const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
+    int best_mi = 1, best_ni = 1;
+    double best = -1.0;
+    for (int mi = 4; mi >= 1; mi /= 2)
+        for (int ni = 4; ni >= 1; ni /= 2) {
+            const int64_t tm = (M + 64 * mi - 1) / (64 * mi), tn = (N + 64 * ni - 1) / (64 * ni);
+            const double tiles = (double)tm * tn * batch;
+            const double edge = ((double)M * N) / ((double)tm * 64 * mi * tn * 64 * ni);
+            const double waves = std::ceil(tiles / cus);
+            const double util = tiles / (waves * cus);
+            const double reuse = 1.0 / (1.0 / (64.0 * mi) + 1.0 / (64.0 * ni)) / 128.0;   // 1 for 256 x 256
+            const double score = edge * util * (0.55 + 0.45 * reuse);
+            if (score > best) { best = score; best_mi = mi; best_ni = ni; }
+        }
+    // the caller's tile, if it names one (tile_m x tile_n of 64, 128 or 256)
+    if (tile_m == 64 || tile_m == 128 || tile_m == 256) best_mi = tile_m / 64;
+    if (tile_n == 64 || tile_n == 128 || tile_n == 256) best_ni = tile_n / 64;
+    // Few tiles and a long sum: the sum is cut into slices, whose float32 results a reduce launch adds up.  A stage (32 float32 or 64
+    // 16-bit elements of the sum) of a 64 x 64 tile takes about 0.75 us in float32 and 0.5 in 16 bits with a compute unit to itself, 1.75 / 2.6 / 3.4 times that
+    // with two / three / four workgroups a unit; the reduce launch 5 us and its traffic.  At most 16 slices: their reduce is
+    // a single launch, which leaves the scratch memory alone.  (us whole / in slices; a^T b: 512 x 512 x 8192 float32
+    // 183 / 50, bfloat16 64.5 / 22.7; 64 x 64 x 4096 float32 94 / 13.5; 1024 x 512 x 4096 float32 96 / 50; a b^T:
+    // 256 x 1024 x 1024 float32 20.1 / 12.4; 1024 x 1024 x 2048 a^T b, 256 tiles, 50.4 / 50.6, stays whole.)
+    const int64_t ks = esz == 2 ? 64 : 32, stages = (K + ks - 1) / ks;
+    int64_t slices = 1, per = stages;
+    bool split = false;
+    const bool sliceable = batch == 1 && !tile_m && !tile_n && ldc == N;
+    const double tiles64 = (double)((M + 63) / 64) * ((N + 63) / 64) * batch;
+    auto crowd = [&](double wgs) { const double r = std::ceil(wgs / cus); return 1.0 + 0.8 * (r - 1.0); };
+    const double st = esz == 2 ? 0.5 : 0.75;
+    double least = (double)stages * st * crowd(tiles64) * (best_mi * best_ni > 1 ? 0.95 : 1.0);
+    // float32 sums of four stages and more go as products of bfloat16 parts (kernels/gemm_mfma.h) on 128 x 64, 64 x 128 or
+    // 128 x 128 tiles, whole or in slices, where that is estimated to take less.  A stage takes 0.92 us on 128 x 64 tiles and 1.45
+    // on 128 x 128, a little more where an operand is transposed on the way; a round of workgroups adds a first load and a
+    // store that nothing overlaps.  64 x 64 tiles stay with the float32 MFMAs: their stage is bound by the splitting (46 to
+    // 56 us / 52 to 57 for a^T b 1024 x 1024 x 2048, 17.1 / 15.7 for a b^T 8192 x 64 x 1024).
+    // us, float32 MFMAs on the tiles chosen before / so: a b^T 2048 x 1024 x 1024 38.4 / 31.5 (128 x 64), a b 40.0 / 31.7, a^T b 1024 x
+    // 1024 x 2048 50.3 / 36.7 (128 x 128, 4 slices), a b^T 2048^3 126 / 92.5 (128 x 128), 4096^3 966 / 703, 512 x 512 x 8192 a^T b
+    // 51 / 35.4, 64 x 512 x 512 x 256 143 / 65.5, 12 x 384 x 384 x 384 35.5 / 17.2.
+    const bool parts = in_dtype == MJT_FLOAT32 && stages >= 4;
+    for (int t = 0; t < (parts ? 4 : 1); t++) {
+        const int mi = t == 1 || t == 3 ? 2 : 1, ni = t >= 2 ? 2 : 1;
+        const double tiles = (double)((M + 64 * mi - 1) / (64 * mi)) * ((N + 64 * ni - 1) / (64 * ni)) * batch;
+        for (int64_t n = t ? 1 : 2; n == 1 || (sliceable && n <= 16 && n <= stages / 4); n++) {
+            const int64_t pn = (stages + n - 1) / n, nn = (stages + pn - 1) / pn;
+            const double rounds = std::ceil(tiles * nn / cus);
+            double us = t ? (nn > 1 ? 4.0 + (double)nn * M * N * 8 / 4.5e6 : -2.0) : nn > 1 ? 5.0 + (double)nn * M * N * 8 / 3e6 : 0.0;
+            if (t == 0) us = (us + (double)pn * st * crowd(tiles * nn)) / 0.9;
+            else if (t == 3) us += rounds * ((double)pn * (a_kcont && b_kcont ? 1.45 : 1.55) + 6.5);
+            else us += rounds * ((double)pn * (a_kcont && b_kcont ? 0.92 : 1.05) * (rounds > 1 ? 0.9 : 1.0) * (t == 2 ? 1.06 : 1.0) + 3.5);
+            if (us < least && (nn == 1 || nn * M * N * 4 <= (int64_t(256) << 20))) {
+                least = us; slices = nn; per = pn; split = t > 0; best_mi = mi; best_ni = ni;
+            }
+        }
+    }
+    return {best_mi, best_ni, slices, per, stages, split};
+}
+
 // One strided-batched product C[b] = A'[b] * B'[b] over plain pointers: M x K times K x N, leading dimensions and
 // batch strides in elements (a batch stride of 0 shares the operand).  a_kcont / b_kcont: the operand's memory has
 // k innermost (a as given, b transposed).
@@ -161,63 +230,11 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
         }
     }
     if (fast) {
-        // Tile: the largest of 64 MI x 64 NI (MI, NI in 1, 2, 4) that still gives every compute unit work and wastes
-        // little on the edges; larger tiles read each operand element less often.
-        const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
-        int best_mi = 1, best_ni = 1;
-        double best = -1.0;
-        for (int mi = 4; mi >= 1; mi /= 2)
-            for (int ni = 4; ni >= 1; ni /= 2) {
-                const int64_t tm = (M + 64 * mi - 1) / (64 * mi), tn = (N + 64 * ni - 1) / (64 * ni);
-                const double tiles = (double)tm * tn * batch;
-                const double edge = ((double)M * N) / ((double)tm * 64 * mi * tn * 64 * ni);
-                const double waves = std::ceil(tiles / cus);
-                const double util = tiles / (waves * cus);
-                const double reuse = 1.0 / (1.0 / (64.0 * mi) + 1.0 / (64.0 * ni)) / 128.0;   // 1 for 256 x 256
-                const double score = edge * util * (0.55 + 0.45 * reuse);
-                if (score > best) { best = score; best_mi = mi; best_ni = ni; }
-            }
-        // the caller's tile, if it names one (tile_m x tile_n of 64, 128 or 256)
-        if (tile_m == 64 || tile_m == 128 || tile_m == 256) best_mi = tile_m / 64;
-        if (tile_n == 64 || tile_n == 128 || tile_n == 256) best_ni = tile_n / 64;
-        // Few tiles and a long sum: the sum is cut into slices, whose float32 results a reduce launch adds up.  A stage (32 float32 or 64
-        // 16-bit elements of the sum) of a 64 x 64 tile takes about 0.75 us in float32 and 0.5 in 16 bits with a compute unit to itself, 1.75 / 2.6 / 3.4 times that
-        // with two / three / four workgroups a unit; the reduce launch 5 us and its traffic.  At most 16 slices: their reduce is
-        // a single launch, which leaves the scratch memory alone.  (us whole / in slices; a^T b: 512 x 512 x 8192 float32
-        // 183 / 50, bfloat16 64.5 / 22.7; 64 x 64 x 4096 float32 94 / 13.5; 1024 x 512 x 4096 float32 96 / 50; a b^T:
-        // 256 x 1024 x 1024 float32 20.1 / 12.4; 1024 x 1024 x 2048 a^T b, 256 tiles, 50.4 / 50.6, stays whole.)
-        const int64_t ks = esz == 2 ? 64 : 32, stages = (K + ks - 1) / ks;
-        int64_t slices = 1, per = stages;
-        bool split = false;
-        const bool sliceable = batch == 1 && !tile_m && !tile_n && ldc == N;
-        const double tiles64 = (double)((M + 63) / 64) * ((N + 63) / 64) * batch;
-        auto crowd = [&](double wgs) { const double r = std::ceil(wgs / cus); return 1.0 + 0.8 * (r - 1.0); };
-        const double st = esz == 2 ? 0.5 : 0.75;
-        double least = (double)stages * st * crowd(tiles64) * (best_mi * best_ni > 1 ? 0.95 : 1.0);
-        // float32 sums of four stages and more go as products of bfloat16 parts (kernels/gemm_mfma.h) on 128 x 64, 64 x 128 or
-        // 128 x 128 tiles, whole or in slices, where that is estimated to take less.  A stage takes 0.92 us on 128 x 64 tiles and 1.45
-        // on 128 x 128, a little more where an operand is transposed on the way; a round of workgroups adds a first load and a
-        // store that nothing overlaps.  64 x 64 tiles stay with the float32 MFMAs: their stage is bound by the splitting (46 to
-        // 56 us / 52 to 57 for a^T b 1024 x 1024 x 2048, 17.1 / 15.7 for a b^T 8192 x 64 x 1024).
-        // us, float32 MFMAs on the tiles chosen before / so: a b^T 2048 x 1024 x 1024 38.4 / 31.5 (128 x 64), a b 40.0 / 31.7, a^T b 1024 x
-        // 1024 x 2048 50.3 / 36.7 (128 x 128, 4 slices), a b^T 2048^3 126 / 92.5 (128 x 128), 4096^3 966 / 703, 512 x 512 x 8192 a^T b
-        // 51 / 35.4, 64 x 512 x 512 x 256 143 / 65.5, 12 x 384 x 384 x 384 35.5 / 17.2.
-        const bool parts = in_dtype == MJT_FLOAT32 && stages >= 4;
-        for (int t = 0; t < (parts ? 4 : 1); t++) {
-            const int mi = t == 1 || t == 3 ? 2 : 1, ni = t >= 2 ? 2 : 1;
-            const double tiles = (double)((M + 64 * mi - 1) / (64 * mi)) * ((N + 64 * ni - 1) / (64 * ni)) * batch;
-            for (int64_t n = t ? 1 : 2; n == 1 || (sliceable && n <= 16 && n <= stages / 4); n++) {
-                const int64_t pn = (stages + n - 1) / n, nn = (stages + pn - 1) / pn;
-                const double rounds = std::ceil(tiles * nn / cus);
-                double us = t ? (nn > 1 ? 4.0 + (double)nn * M * N * 8 / 4.5e6 : -2.0) : nn > 1 ? 5.0 + (double)nn * M * N * 8 / 3e6 : 0.0;
-                if (t == 0) us = (us + (double)pn * st * crowd(tiles * nn)) / 0.9;
-                else if (t == 3) us += rounds * ((double)pn * (a_kcont && b_kcont ? 1.45 : 1.55) + 6.5);
-                else us += rounds * ((double)pn * (a_kcont && b_kcont ? 0.92 : 1.05) * (rounds > 1 ? 0.9 : 1.0) * (t == 2 ? 1.06 : 1.0) + 3.5);
-                if (us < least && (nn == 1 || nn * M * N * 4 <= (int64_t(256) << 20))) {
-                    least = us; slices = nn; per = pn; split = t > 0; best_mi = mi; best_ni = ni;
-                }
-            }
-        }
+        const TileChoice chosen = choose_tiles(in_dtype, M, N, K, batch, a_kcont, b_kcont, tile_m, tile_n, ldc);
+        const int best_mi = chosen.mi, best_ni = chosen.ni;
+        int64_t slices = chosen.slices;
+        const int64_t per = chosen.per, stages = chosen.stages;
+        const bool split = chosen.split;
         void* part_mem = slices > 1 ? scratch_if_any((size_t)(slices * M * N * 4)) : nullptr;
         if (!part_mem) slices = 1;
         const int MI = best_mi, NI = best_ni;
@@ -280,6 +297,27 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
     }
     MJT_CHECK(batch < 65536 && (M + 63) / 64 < 65536, "matmul: launch too large");
     jit_launch(k, (unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64), 256, 0, args, (unsigned)batch);
+}
+
+bool gemm_gated(int dtype, int act, const char* act_name, const void* x, const void* w, void* y, void* both, int64_t M, int64_t F, int64_t K) {
+    const int esz = dtype_size(dtype);
+    TileChoice t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 2 * F);
+    if (t.slices > 1) return false;
+    t.mi = std::min(t.mi, 2);                                   // (a tile's results have to fit its LDS)
+    t.ni = std::min(t.ni, 2);
+    const int in = dtype == MJT_BFLOAT16 ? 0 : dtype == MJT_FLOAT16 ? 1 : 2, gated = (y ? 1 : 0) + (both ? 2 : 0);
+    const bool one_stage = t.stages == 1 && t.mi * t.ni == 1;
+    const int vs = F % 4 == 0 && (uintptr_t)y % (size_t)(4 * esz) == 0 && (uintptr_t)both % 16 == 0 ? 4 : 1;
+    std::ostringstream name, defs;
+    name << "mjt_gated_mfma_" << act_name << "_" << mjt_dtype_name(dtype) << "_" << 64 * t.mi << "x" << 64 * t.ni << (one_stage ? "_k1" : "") << (t.split ? "_parts" : "") << (both ? y ? "_both" : "_products" : "");
+    defs << "#define NBUF " << (one_stage ? 1 : 2) << "\n#define SPLIT " << (t.split ? 1 : 0) << "\n#define IN " << in << "\n#define OUT 2\n#define MI " << t.mi << "\n#define NI " << t.ni
+         << "\n#define A_KCONT 1\n#define B_KCONT 1\n#define GATED " << gated << "\n#define VS " << vs << "\n#define ACT " << act << "\n";
+    JitKernel* k = t.split ? layer_kernel(name.str(), {"element.h", "gated_act.h", "split.h", "gemm_mfma.h"}, defs.str()) : layer_kernel(name.str(), {"element.h", "gated_act.h", "gemm_mfma.h"}, defs.str());
+    const int64_t tiles = ((M + 64 * t.mi - 1) / (64 * t.mi)) * ((F + 32 * t.ni - 1) / (32 * t.ni)), grid = (tiles + 7) / 8 * 8;
+    MJT_CHECK(grid < (int64_t(1) << 23), "gated_linear: launch too large");
+    jit_launch(k, (unsigned)grid, 1, product_threads(t.split), 0,
+               {bits_of_ptr(x), bits_of_ptr(w), bits_of_ptr(y), (uint64_t)M | uint64_t(1) << 32, (uint64_t)F, (uint64_t)K, (uint64_t)K, bits_of_ptr(both), 0, 0, 0, 0});
+    return true;
 }
 
 // 1x1 convolution of stride 1 over a batch of planes that need not be 16-byte multiples (kernels/gemm_dma.h with IMG):

@@ -441,3 +441,31 @@ def test_products_rounded_to_nearest(gpu, m, k, n, ta, tb):
     L.check(L.load().mjt_matmul_nearest(*[ctypes.byref(u) for u in t], ta, tb))
     x, y = ae.T if ta else ae, be.T if tb else be
     _check(bf16_bits_to_f32(L.d2h(c._buf.ptr, c.shape, np.uint16)).astype(np.float64), x @ y, (k + 2) * E * (np.abs(x) @ np.abs(y)), "bfloat16", "c")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("route,shapes", [("few", [(1, 8, 8), (16, 264, 100), (5, 4104, 24), (7, 512, 9)]),
+                                          ("tiles", [(1, 64, 1), (130, 72, 70), (257, 320, 129), (90, 1000, 200)]),
+                                          ("mfma", [(1, 8, 1), (65, 40, 33), (130, 200, 130), (200, 1032, 260), (64, 64, 64)]),
+                                          ("product", [(3, 40, 24), (130, 264, 70)])])
+def test_every_route_of_gated_projections(gpu, monkeypatch, dtype, route, shapes):
+    """Each kernel on sizes that fill its tiles badly, whichever the sizes would go to."""
+    monkeypatch.setenv("MJT_GATED", route)
+    for tile in ("128", "256") if route == "tiles" else ("",):
+        if tile:
+            monkeypatch.setenv("MJT_GEMM_DMA", tile)
+        for rows, k, f in shapes:
+            k = max(k, 64) if route == "tiles" else k
+            rng = np.random.default_rng(rows)
+            (x, xe), (w, we) = _make(rng, (rows, k), dtype), _make(rng, (2 * f, k), dtype, 1.5 / k ** 0.5)
+            want, off = P.gated(xe, we, "silu")
+            y = jt.nn.gated_linear(x, w)
+            _check(_got(y), want, off, dtype, (route, tile, rows, k, f))
+            if route == "few" or route == "tiles" and dtype != "float32":
+                assert gpu.last_kernel().startswith("mjt_gated_" + route), gpu.last_kernel()
+            y = jt.nn.gated_linear(x, w)
+            both = core._graph.kernel_var(core.KernelOp, y._op.call, 1, [x, w], [rows, 2 * f], "float32")
+            both.sync()                                     # gate and up alone
+            _check(_got(both), xe @ we.T, (k + 2) * E * (np.abs(xe) @ np.abs(we).T), "float32", (route, tile, rows, k, f))
+            jt.sync([y])
+            _check(_got(y), want, off, dtype, (route, tile, rows, k, f))
