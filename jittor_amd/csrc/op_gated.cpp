@@ -58,9 +58,9 @@ Route choose(int dtype, int64_t M, int64_t F, int64_t K, bool aligned, int* tile
     auto tiles_of = [&](int64_t rows, int64_t cols) { return (double)((M + rows - 1) / rows) * (double)((F + cols - 1) / cols); };
     if (may("few") && M <= 16 && (forced || esz == 4 || M <= 4 || 2 * F * K * esz <= int64_t(24) << 20)) return FEW;
     if (may("tiles") && esz == 2 && K >= 64 && K * 2 * 256 < (int64_t(1) << 31)) {
-        const double r256 = rounds(tiles_of(256, 128), (double)cus), n128 = tiles_of(128, 64);
+        const double r256 = rounds(tiles_of(256, 128), (double)cus), n128 = tiles_of(128, 64), r128 = rounds(n128, 2.0 * (double)cus);
         const double t256 = r256 * (10.0 + 1.1 * stages) * (r256 > 1 ? 1.2 : 1.0);
-        const double t128 = n128 <= (double)cus ? 5.3 + 0.335 * stages : rounds(n128, 2.0 * (double)cus) * (6.0 + 0.66 * stages * (1.0 + std::max(0.0, stages - 32.0) / 64.0));
+        const double t128 = n128 <= (double)cus ? 5.3 + 0.335 * stages : r128 * (6.0 + 0.66 * stages * (1.0 + std::max(0.0, stages - 32.0) / 64.0)) * (r128 > 1 && stages >= 32.0 ? 1.2 : 1.0);
         const double mfma = 3.5 + 0.25 * stages * (1.0 + 0.8 * (rounds(tiles_of(64, 32), (double)cus) - 1.0));
         *tile = t256 < t128 ? 256 : 128;
         if (const char* e = getenv("MJT_GEMM_DMA")) *tile = atoi(e) == 128 ? 128 : 256;

@@ -22,7 +22,7 @@ struct Plan {
 
 // Checks what both directions have in common and chooses vectors and lanes.  `parts`: q, k and v or their gradients (null: left out).
 Plan plan_for(const char* who, const mjt_tensor* x, const mjt_tensor* q_scale, const mjt_tensor* k_scale, const mjt_tensor* table, const mjt_tensor* positions,
-              const mjt_head_norm* p, const mjt_tensor* const parts[3], const mjt_tensor* dx) {
+              const mjt_head_norm* p, const mjt_tensor* const parts[3], const mjt_tensor* dx, bool back) {
     require_init();
     MJT_CHECK(p, who << ": null parameters");
     check_tensor(x, who);
@@ -96,9 +96,11 @@ Plan plan_for(const char* who, const mjt_tensor* x, const mjt_tensor* q_scale, c
         MJT_CHECK(n == axes * a.tokens || n == axes * S, who << ": " << n << " positions for " << axes << " axes of " << a.tokens << " tokens in sequences of " << S);
         per = n / axes;
     }
-    // vectors: 16 bytes where pairs, rows and pointers allow
+    // Vectors of 16 bytes where pairs, rows and pointers allow; of 16-bit elements 8 bytes in the backward pass and with several axes, where eight
+    // pairs a lane take more registers than the wider access gives back (us for 8 / 4 pairs: 48 heads of 128, 8192 tokens, forward 41.4 / 44.8,
+    // backward 64.2 / 63.3; 24 heads of 80 on three axes, 9477 tokens, 21.9 / 18.0 and 41.8 / 30.5).
     const int esz = dtype_size(x->dtype), ssz = q_scale ? dtype_size(q_scale->dtype) : 1;
-    int V = 16 / esz;
+    int V = back || axes > 1 ? 4 : 16 / esz;
     auto fits = [&](int v) {
         if ((rot / 2) % v || (D / 2) % v) return false;
         for (const mjt_tensor* t : {x, parts[0], parts[1], parts[2], dx})
@@ -129,19 +131,20 @@ Plan plan_for(const char* who, const mjt_tensor* x, const mjt_tensor* q_scale, c
 void forward(const mjt_tensor* x, const mjt_tensor* q_scale, const mjt_tensor* k_scale, const mjt_tensor* table, const mjt_tensor* positions, const mjt_head_norm* p, const mjt_tensor* q,
              const mjt_tensor* k, const mjt_tensor* v) {
     const mjt_tensor* parts[3] = {q, k, v};
-    Plan a = plan_for("head_norm_rope", x, q_scale, k_scale, table, positions, p, parts, nullptr);
+    Plan a = plan_for("head_norm_rope", x, q_scale, k_scale, table, positions, p, parts, nullptr, false);
     if (a.tokens == 0 || a.heads == 0) return;
-    const int rows = 64 / a.LP;
-    const int IT = 1;
-    JitKernel* kern = layer_kernel(a.name, {"element.h", "head_norm_rope.h"}, a.defines + "#define BACK 0\n#define SUMS 0\n#define IT " + std::to_string(IT) + "\n");
-    const int64_t across = (a.heads + rows * IT - 1) / (rows * IT), along = (a.tokens + 3) / 4;
-    jit_launch(kern, (unsigned)std::min(along, int64_t(1) << 20), (unsigned)std::min<int64_t>(across, 64), 256, 0, a.args);
+    const int64_t rows = 64 / a.LP, rounds = (p->q_heads + rows - 1) / rows + (p->k_heads + rows - 1) / rows + (p->v_heads + rows - 1) / rows;
+    // Few tokens: a wave for every round of every token.  Many: a wave for a token, three rounds under way together (us for 1 / 2 / 3 / 6 rounds: 48
+    // heads of 128, 8192 tokens 47.1 / 43.3 / 41.4 / 45.3; 24 heads of 80, 9477 tokens 20.9 / 19.0 / 18.0 / 18.3).
+    const bool few = a.tokens * rounds <= 4096;
+    JitKernel* kern = layer_kernel(a.name, {"element.h", "head_norm_rope.h"}, a.defines + "#define BACK 0\n#define SUMS 0\n#define IT " + (few ? "1" : "3") + "\n");
+    jit_launch(kern, (unsigned)std::min((a.tokens + 3) / 4, int64_t(1) << 20), few ? (unsigned)rounds : 1, 256, 0, a.args);
 }
 
 void backward(const mjt_tensor* x, const mjt_tensor* q_scale, const mjt_tensor* k_scale, const mjt_tensor* table, const mjt_tensor* positions, const mjt_head_norm* p, const mjt_tensor* dq,
               const mjt_tensor* dk, const mjt_tensor* dv, const mjt_tensor* dx, const mjt_tensor* dq_scale, const mjt_tensor* dk_scale) {
     const mjt_tensor* parts[3] = {dq, dk, dv};
-    Plan a = plan_for("head_norm_rope_grad", x, q_scale, k_scale, table, positions, p, parts, dx);
+    Plan a = plan_for("head_norm_rope_grad", x, q_scale, k_scale, table, positions, p, parts, dx, true);
     const bool sums = dq_scale || dk_scale;
     for (const mjt_tensor* s : {dq_scale, dk_scale})
         if (s) {
@@ -160,12 +163,12 @@ void backward(const mjt_tensor* x, const mjt_tensor* q_scale, const mjt_tensor* 
     if (!nothing) {
         a.args[16] = bits_of_ptr(dx ? dx->ptr : nullptr);
         a.args[17] = bits_of_ptr(part);
-        JitKernel* kern = layer_kernel(a.name + "_grad", {"element.h", "head_norm_rope.h"}, a.defines + "#define BACK 1\n#define SUMS " + (sums ? "1" : "0") + "\n#define IT 1\n");
+        JitKernel* kern = layer_kernel(a.name + "_grad", {"element.h", "head_norm_rope.h"}, a.defines + "#define BACK 1\n#define SUMS " + (sums ? "1" : "0") + "\n#define IT 3\n");
         jit_launch(kern, (unsigned)blocks, 1, 256, 0, a.args);
     }
     if (!sums) return;
     JitKernel* fold = layer_kernel("mjt_head_norm_rope_fold", {"element.h", "head_norm_rope.h"}, "#define FOLD 1\n#define STYPE " + std::to_string(a.scale_type) + "\n");
-    jit_launch(fold, (unsigned)((2 * a.dim + 31) / 32), 1, 1024, 0,
+    jit_launch(fold, (unsigned)((2 * a.dim + 15) / 16), 1, 1024, 0,
                {bits_of_ptr(part), bits_of_ptr(dq_scale ? dq_scale->ptr : nullptr), bits_of_ptr(dk_scale ? dk_scale->ptr : nullptr), (uint64_t)blocks, (uint64_t)a.dim});
 }
 }  // namespace
