@@ -647,15 +647,30 @@ bool in_set(PyObject* set, PyObject* v) {
     return i && PySet_Contains(set, i) == 1;
 }
 bool is_text(PyObject* s, const char* t) { return s && PyUnicode_Check(s) && PyUnicode_CompareWithASCIIString(s, t) == 0; }
+// A Var of its own with the value of a number's shared one: what array(number, dtype) makes, without converting the number again.
+PyObject* own_number(PyObject* shared) {
+    PyObject* host = own(shared, s__host);
+    PyObject* dtype = own(shared, s_dtype);
+    if (!host || host == Py_None || !dtype) { PyErr_SetString(PyExc_RuntimeError, "a number without its value"); return nullptr; }
+    PyObject* d;
+    Ref v(instance(t_var, &d));
+    if (!v || !put(d, s_shape, Py_BuildValue("[i]", 1)) || !put(d, s_num, PyLong_FromLong(1)) || PyDict_SetItem(d, s_dtype, dtype) || PyDict_SetItem(d, s__op, Py_None) ||
+        PyDict_SetItem(d, s__history, Py_None) || !put(d, s_id, PyLong_FromLongLong(g_next_id++)) || PyDict_SetItem(d, s__host, host) || PyDict_SetItem(d, s_is_scalar, Py_True))
+        return nullptr;
+    PyObject* co = PyDict_GetItemWithError(g_flags, s_compile_options);
+    if (co && PyObject_IsTrue(co) == 1 && !put(d, s__compile_options, PyObject_CallOneArg((PyObject*)&PyDict_Type, co))) return nullptr;
+    return v.give();
+}
 PyObject* number_like(double value, bool whole, PyObject* like) {
     Shape s;
     Ref dtype = attr(like, s_dtype);
     if (!dtype || !var_shape(like, &s)) return nullptr;
     Ref n(whole ? PyLong_FromLong((long)value) : PyFloat_FromDouble(value));
     if (!n) return nullptr;
-    if (s.n == 1 && s.e[0] == 1) return PyObject_CallFunctionObjArgs(g_array, n.p, dtype.p, nullptr);
     Ref v(number_var(n.p, dtype.p));
-    return v ? broadcast_plain(v.p, s) : nullptr;
+    if (!v) return nullptr;
+    if (s.n == 1 && s.e[0] == 1) return own_number(v.p);
+    return broadcast_plain(v.p, s);
 }
 PyObject *s_multiply, *s_divide, *s_subtract, *s_negative, *s_equal;
 // factor * dout, which is `factor` itself where dout is the seed of this call, spread or cast: the product would be a pass over memory that

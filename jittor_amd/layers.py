@@ -17,15 +17,21 @@ from .core import KernelOp, Var
 _FLOATS = ("float32", "bfloat16", "float16")
 
 
+_numbers = {}            # (name, options) -> its number
+
+
 class Call:
     """What is called and with which options; shared by the ops of its results."""
-    __slots__ = ("name", "options")
+    __slots__ = ("name", "options", "number")
 
     def __init__(self, name, *options):
-        self.name, self.options = name, options
+        self.name, self.options, self.number = name, options, None
 
     def key(self):
-        return (self.name,) + self.options
+        """A number for name and options: a graph's key is worked out and looked up for every execution."""
+        if self.number is None:
+            self.number = _numbers.setdefault((self.name, self.options), len(_numbers))
+        return self.number
 
 
 def _result(call, index, inputs, shape, dtype):
