@@ -168,17 +168,7 @@ class _Pool:
 pool = _Pool()
 
 
-class Buffer:
-    """Owns one device allocation."""
-
-    def __init__(self, nbytes):
-        self.ptr, self.size = pool.alloc(nbytes)
-
-    def __del__(self):
-        try:
-            pool.free(self.ptr, self.size)
-        except Exception:
-            pass
+Buffer = _graph.Buffer         # Buffer(nbytes): owns one device allocation of the pool's, `ptr` of `size` bytes (csrc/py/graph.cpp)
 
 
 # --------------------------------------------------------------------------

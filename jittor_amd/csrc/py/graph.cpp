@@ -10,6 +10,7 @@
 // of 12 element ops 58 / 22).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <structmember.h>
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -38,7 +39,7 @@ struct Ref {
 PyObject* keep(PyObject* p) { Py_XINCREF(p); return p; }
 
 #define NAMES(X) X(shape) X(num) X(dtype) X(_op) X(_history) X(id) X(_out_ref) X(inputs) X(amp) X(op) X(bcast_mask) X(keepdims_mask) X(reduce_mask) X(is_scalar) \
-    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) X(call) X(index) X(ptr) X(_device_ptr) X(int64) X(int32) \
+    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) X(call) X(index) X(_device_ptr) X(int64) X(int32) \
     X(_binary_dtypes) X(binary_dtype_infer) X(unary_dtype_infer) X(reduce_dtype_infer) X(dtype_infer) X(cast) X(add) X(mean) X(float16) X(bfloat16) X(float32)
 #define DECLARE(n) PyObject* s_##n;
 NAMES(DECLARE)
@@ -1109,6 +1110,130 @@ PyObject* py_signature(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return rest ? PyTuple_Pack(2, bytes.p, rest.p) : nullptr;
 }
 
+// ---- device buffers ---------------------------------------------------------------------------------------------------------------
+// core.Buffer: owns one device allocation, a block of core.pool.  Taking a block of a size that the pool has, and giving one back to a pool
+// with room, is done here on the pool's own tables and under its lock (1.6 us for the two in byte code, 0.4 here; every result of
+// every call has one); whatever else there is to do is the pool's: a driver call, a full pool, bookkeeping under way, methods
+// replaced on the instance.
+struct Buffer {
+    PyObject_HEAD
+    PyObject *ptr, *size;
+};
+PyObject *g_core = nullptr, *g_lib = nullptr;                  // the dictionaries of core.py and _lib.py
+PyObject* g_pool_type = nullptr;
+PyObject *s_pool, *s_alloc, *s_free, *s__enter, *s__leave, *s__inside, *s_free_blocks, *s_cached_bytes, *s_limit, *s__device;
+
+struct Pool {
+    PyObject *pool, *d, *blocks = nullptr;
+    bool held = false;
+    // d: the pool's instance dictionary where it can be worked on here, its lock held; null otherwise
+    explicit Pool(PyObject* method) : pool(PyDict_GetItem(g_core, s_pool)), d(nullptr) {
+        if (!pool || (PyObject*)Py_TYPE(pool) != g_pool_type) return;
+        PyObject* own_dict = dict_of(pool);
+        PyObject* enter = own_dict ? PyDict_GetItem(own_dict, s__enter) : nullptr;
+        if (!enter || PyDict_GetItem(own_dict, method)) return;
+        Ref got(PyObject_CallOneArg(enter, Py_False));         // without waiting; from here on no Python code runs
+        if (got.p != Py_True) {
+            PyErr_Clear();
+            return;
+        }
+        held = true;
+        blocks = PyDict_GetItem(own_dict, s_free_blocks);
+        if (blocks && PyDict_CheckExact(blocks) && PyDict_GetItem(own_dict, s__inside) == Py_False) d = own_dict;
+        else leave(own_dict);
+    }
+    void leave(PyObject* own_dict) {
+        if (!held) return;
+        held = false;
+        PyObject* f = PyDict_GetItem(own_dict, s__leave);
+        Ref r(f ? PyObject_CallNoArgs(f) : nullptr);
+        if (!r) PyErr_Clear();
+    }
+    ~Pool() { if (d) leave(d); }
+    long long number(PyObject* name) {
+        PyObject* v = PyDict_GetItem(d, name);
+        return v ? PyLong_AsLongLong(v) : -1;
+    }
+};
+long long rounded(long long n) {                               // _Pool._round
+    if (n <= 256) return 256;
+    if (n > 1 << 20) return (n + (1 << 20) - 1) >> 20 << 20;
+    long long r = 512;
+    while (r < n) r <<= 1;
+    return r;
+}
+PyObject* buffer_new(PyTypeObject* type, PyObject* args, PyObject* kw) {
+    if (!g_core) return PyErr_Format(PyExc_RuntimeError, "a buffer before setup()");
+    PyObject* nbytes;
+    static const char* names[] = {"nbytes", nullptr};
+    if (!PyArg_ParseTupleAndKeywords(args, kw, "O", (char**)names, &nbytes)) return nullptr;
+    Ref self(type->tp_alloc(type, 0));
+    if (!self) return nullptr;
+    Buffer* b = (Buffer*)self.p;
+    const long long n = PyLong_AsLongLong(nbytes);
+    if (n == -1 && PyErr_Occurred()) return nullptr;
+    Ref size(PyLong_FromLongLong(rounded(n)));
+    if (!size) return nullptr;
+    {
+        Pool pool(s_alloc);
+        PyObject* list = pool.d ? PyDict_GetItem(pool.blocks, size.p) : nullptr;
+        const Py_ssize_t have = list && PyList_CheckExact(list) ? PyList_GET_SIZE(list) : 0;
+        if (have) {
+            Ref left(PyLong_FromLongLong(pool.number(s_cached_bytes) - rounded(n)));
+            Ref last(keep(PyList_GET_ITEM(list, have - 1)));
+            if (!left || PyList_SetSlice(list, have - 1, have, nullptr) || (have == 1 && PyDict_DelItem(pool.blocks, size.p)) || PyDict_SetItem(pool.d, s_cached_bytes, left.p)) return nullptr;
+            b->ptr = last.give();
+            b->size = size.give();
+            return self.give();
+        }
+    }
+    PyObject* pool = PyDict_GetItem(g_core, s_pool);
+    Ref got(pool ? PyObject_CallMethodOneArg(pool, s_alloc, nbytes) : nullptr);
+    if (!got) {
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "there is no pool");
+        return nullptr;
+    }
+    if (!PyTuple_Check(got.p) || PyTuple_GET_SIZE(got.p) != 2) return PyErr_Format(PyExc_TypeError, "pool.alloc returns (ptr, size)");
+    b->ptr = keep(PyTuple_GET_ITEM(got.p, 0));
+    b->size = keep(PyTuple_GET_ITEM(got.p, 1));
+    return self.give();
+}
+// true: the block is in the pool
+bool give_back(Buffer* b) {
+    const long long size = PyLong_AsLongLong(b->size);
+    Ref fresh(PyList_New(0));                                  // (may start a collection: before anything is looked at)
+    Pool pool(s_free);
+    if (!fresh || !pool.d || size <= 0) return false;
+    const long long cached = pool.number(s_cached_bytes), limit = pool.number(s_limit);
+    if (cached < 0 || limit < 0 || cached + size > limit) return false;
+    PyObject* list = PyDict_GetItem(pool.blocks, b->size);
+    Ref held(list ? keep(list) : fresh.give()), total(PyLong_FromLongLong(cached + size));
+    if (!PyList_CheckExact(held.p) || !total || PyList_Append(held.p, b->ptr)) return false;
+    // the size used last goes to the end
+    if ((list && PyDict_DelItem(pool.blocks, b->size)) || PyDict_SetItem(pool.blocks, b->size, held.p) || PyDict_SetItem(pool.d, s_cached_bytes, total.p)) PyErr_Clear();
+    return true;
+}
+void buffer_dealloc(PyObject* self) {
+    Buffer* b = (Buffer*)self;
+    if (b->ptr && b->size) {
+        PyObject *et, *ev, *tb;
+        PyErr_Fetch(&et, &ev, &tb);
+        PyObject* device = PyDict_GetItem(g_lib, s__device);
+        if (device && device != Py_None && !give_back(b)) {
+            PyErr_Clear();
+            PyObject* pool = PyDict_GetItem(g_core, s_pool);
+            Ref done(pool ? PyObject_CallMethodObjArgs(pool, s_free, b->ptr, b->size, nullptr) : nullptr);
+        }
+        PyErr_Clear();
+        PyErr_Restore(et, ev, tb);
+    }
+    Py_XDECREF(b->ptr);
+    Py_XDECREF(b->size);
+    Py_TYPE(self)->tp_free(self);
+}
+PyMemberDef buffer_members[] = {{"ptr", T_OBJECT, offsetof(Buffer, ptr), READONLY, nullptr}, {"size", T_OBJECT, offsetof(Buffer, size), READONLY, nullptr}, {nullptr, 0, 0, 0, nullptr}};
+PyTypeObject buffer_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+
 // ---- replays --------------------------------------------------------------------------------------------------------------------
 // A plan of the executor whose launches are recorded (executor.py: _Plan, _replay): gives the results of a graph their buffers and
 // issues the recording, as _replay does in byte code (us of host time a pass, there / here: one launch with three results 13.5 / 8.3, two with two 17.9 / 12.0).
@@ -1223,7 +1348,7 @@ PyObject* py_replay(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         return PyList_GET_ITEM(ops, i);
     };
     auto address = [&](size_t k) {                             // of the buffer in buf[k]
-        PyObject* p = own(buf[k].p, s_ptr);
+        PyObject* p = Py_TYPE(buf[k].p) == &buffer_type ? ((Buffer*)buf[k].p)->ptr : nullptr;
         base[k] = p ? (uint64_t)PyLong_AsUnsignedLongLong(p) : 0;
         if (!p) PyErr_SetString(PyExc_AttributeError, "a buffer without an address");
         return p && !PyErr_Occurred();
@@ -1336,6 +1461,11 @@ PyObject* py_setup(PyObject*, PyObject* ns) {
         *w.to = keep(v);
         Py_XDECREF(old);
     }
+    PyObject *lib = PyDict_GetItemString(ns, "_lib"), *pool = PyDict_GetItemString(ns, "_Pool");
+    if (!lib || !PyModule_Check(lib) || !pool) return PyErr_Format(PyExc_KeyError, "setup: _lib, _Pool");
+    g_core = keep(ns);
+    g_lib = keep(PyModule_GetDict(lib));
+    g_pool_type = keep(pool);
     PyObject* m = PyDict_GetItemString(ns, "_MAX_DIM");
     if (!m) return PyErr_Format(PyExc_KeyError, "setup: _MAX_DIM");
     g_max_dim = PyLong_AsLongLong(m);
@@ -1372,8 +1502,20 @@ PyMODINIT_FUNC PyInit__graph(void) {
 #define INTERN(n) if (!(s_##n = PyUnicode_InternFromString(#n))) return nullptr;
     NAMES(INTERN)
 #undef INTERN
-    struct { PyObject** to; const char* text; } more[] = {{&s_void, "void"}, {&s_multiply, "multiply"}, {&s_divide, "divide"}, {&s_subtract, "subtract"}, {&s_negative, "negative"}, {&s_equal, "equal"}};
+    struct { PyObject** to; const char* text; } more[] = {{&s_void, "void"}, {&s_multiply, "multiply"}, {&s_divide, "divide"}, {&s_subtract, "subtract"}, {&s_negative, "negative"}, {&s_equal, "equal"},
+        {&s_pool, "pool"}, {&s_alloc, "alloc"}, {&s_free, "free"}, {&s__enter, "_enter"}, {&s__leave, "_leave"}, {&s__inside, "_inside"}, {&s_free_blocks, "free_blocks"},
+        {&s_cached_bytes, "cached_bytes"}, {&s_limit, "limit"}, {&s__device, "_device"}};
     for (auto& m : more)
         if (!(*m.to = PyUnicode_InternFromString(m.text))) return nullptr;
-    return PyModule_Create(&module);
+    buffer_type.tp_name = "jittor_amd._graph.Buffer";
+    buffer_type.tp_doc = "Buffer(nbytes): owns one device allocation, ptr of size bytes";
+    buffer_type.tp_basicsize = sizeof(Buffer);
+    buffer_type.tp_flags = Py_TPFLAGS_DEFAULT;
+    buffer_type.tp_new = buffer_new;
+    buffer_type.tp_dealloc = buffer_dealloc;
+    buffer_type.tp_members = buffer_members;
+    if (PyType_Ready(&buffer_type)) return nullptr;
+    Ref m(PyModule_Create(&module));
+    if (!m || PyModule_AddObjectRef(m.p, "Buffer", (PyObject*)&buffer_type)) return nullptr;
+    return m.give();
 }
