@@ -161,6 +161,19 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
                       M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31) && batch < 65536;
     std::vector<uint64_t> args{bits_of_ptr(A), bits_of_ptr(B), bits_of_ptr(C), (uint64_t)M, (uint64_t)N, (uint64_t)K,
                                (uint64_t)lda, (uint64_t)ldb, (uint64_t)ldc, (uint64_t)sa, (uint64_t)sb, (uint64_t)sc};
+    // 256 x 256 tiles that fill some rounds of the compute units and less than 0.7 of another: the whole rounds' tile rows first, and
+    // the rest as a product of its own, on the tiles that suit it (us as one / so: bfloat16 a^T b 11264 x 2048 x 8192, 352 tiles, 350 / 314).  For the products
+    // of layers.py's gradients; others keep the sums they had.
+    if (fast && allow_direct && esz == 2 && Nearest::on() && batch == 1 && K % 64 == 0 && K >= 1024 && !tile_m && !tile_n) {
+        const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
+        const int64_t tn = (N + 255) / 256, tiles = (M + 255) / 256 * tn, rows = tiles / cus * cus / tn * 256;
+        if (tiles > cus && tiles % cus && (double)(tiles % cus) < 0.7 * (double)cus && rows > 0 && rows < M && (double)(rows / 256 * tn) >= 0.95 * (double)(tiles / cus * cus)) {
+            const char* rest = (const char*)A + rows * (a_kcont ? lda : 1) * esz;
+            gemm_launch(in_dtype, out_dtype, A, B, C, rows, N, K, lda, ldb, ldc, sa, sb, sc, 1, a_kcont, b_kcont);
+            gemm_launch(in_dtype, out_dtype, rest, B, (char*)C + rows * ldc * dtype_size(out_dtype), M - rows, N, K, lda, ldb, ldc, sa, sb, sc, 1, a_kcont, b_kcont);
+            return;
+        }
+    }
     // 16-bit operands, K a multiple of 64 and enough tiles of 256 x 256 to go round: the kernel whose operands reach LDS
     // without passing through registers (any of the four layouts).  Offsets inside an operand's tile are 32-bit there:
     // 256 rows of an operand with k innermost, all K rows of one with m or n innermost.

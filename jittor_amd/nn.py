@@ -270,8 +270,9 @@ def gated_linear(x, weight, activation="silu"):
 
 
 def gated_ffn(x, w_in, w_out, activation="silu"):
-    """The whole feed-forward layer: gated_linear(x, w_in) * w_out^T, w_in [2 f, k], w_out [n, f]."""
-    return matmul_transpose(gated_linear(x, w_in, activation), w_out)
+    """The whole feed-forward layer: gated_linear(x, w_in) * w_out^T, w_in [2 f, k], w_out [n, f], in x's type."""
+    with flag_scope(amp_reg=flags.amp_reg | 36):               # (a sum of 16-bit products keeps their type, as a convolution's does)
+        return matmul_transpose(gated_linear(x, w_in, activation), w_out)
 
 
 core.Var.matmul = core.Var.__matmul__ = matmul

@@ -427,7 +427,7 @@ def test_gated_replays(gpu):
         _check(_got(dw), dwe, dwo, "bfloat16", turn)
 
 
-@pytest.mark.parametrize("m,k,n,ta,tb", [(40, 30, 20, 0, 0), (256, 512, 256, 0, 1), (512, 256, 512, 1, 0), (64, 4096, 64, 1, 0), (7, 33, 9, 0, 1)])
+@pytest.mark.parametrize("m,k,n,ta,tb", [(40, 30, 20, 0, 0), (256, 512, 256, 0, 1), (512, 256, 512, 1, 0), (64, 4096, 64, 1, 0), (7, 33, 9, 0, 1), (9300, 1024, 2048, 1, 0), (9300, 1024, 2048, 0, 0)])
 def test_products_rounded_to_nearest(gpu, m, k, n, ta, tb):
     """mjt_matmul_nearest on each of the product kernels' routes: whole, in slices, plain."""
     import ctypes
@@ -469,3 +469,35 @@ def test_every_route_of_gated_projections(gpu, monkeypatch, dtype, route, shapes
             _check(_got(both), xe @ we.T, (k + 2) * E * (np.abs(xe) @ np.abs(we).T), "float32", (route, tile, rows, k, f))
             jt.sync([y])
             _check(_got(y), want, off, dtype, (route, tile, rows, k, f))
+
+
+# ---- all of them in one model -----------------------------------------------------------------------------------------
+def _example():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "decoder.py")
+    spec = importlib.util.spec_from_file_location("decoder_example", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    return m
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_example_learns_and_continues(gpu, dtype):
+    ex = _example()
+    model, losses, follows = ex.train(steps=60, dtype=dtype)
+    assert losses[0] > 3.0 and losses[-1] < 0.3, (losses[0], losses[-1])
+    out = model.generate(np.arange(4, dtype=np.int32)[:, None], 12)
+    assert all(follows[a] == b for row in out for a, b in zip(row, row[1:]))
+
+
+def test_the_example_token_by_token_is_the_example_at_once(gpu):
+    ex = _example()
+    model = ex.Decoder(seed=3)
+    tokens = np.random.default_rng(0).integers(0, model.vocab, (3, 9))
+    whole = _got(model.forward(tokens))
+    cache = [None] * model.layers
+    for i in range(9):
+        step = _got(model.forward(tokens[:, i:i + 1], cache))
+        # the same sums in other orders: relative to the logits' size, a few hundred roundings of 2^-24
+        assert np.abs(step[:, 0] - whole[:, i]).max() < 512 * E * np.abs(whole).max(), i

@@ -222,3 +222,10 @@ def test_a_key_tells_calls_apart():
         q = jt.nn.qkv_norm_rope(_x(2, 4, 6, 8), 2, 2, _x(8), _x(8), _x(9, 4, 2), **kw)[0]
         return core._graph.signature(core._graph.pending_ops([q]), [q], jt.flags)
     assert key() == key() and len({key(), key(eps=1e-5), key(interleaved=True), key(heads_first=True)}) == 4
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_a_feed_forward_layer_keeps_its_type(dtype):
+    x, w, o = _x(3, 4, dtype=dtype), _x(6, 4, dtype=dtype), _x(5, 3, dtype=dtype)
+    y = jt.nn.gated_ffn(x, w, o)
+    assert y.dtype == dtype and y.shape == [3, 5] and [g.dtype for g in jt.grad(y.sum(), [x, w, o])] == [dtype] * 3
