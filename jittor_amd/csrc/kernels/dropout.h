@@ -71,7 +71,7 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
                 if (RES) add.v[j] = j < have ? res[g * 8 + j] : raw(0);
             }
         }
-        const unsigned keep = mjt_keep_bits((unsigned long long)g, key, call, threshold);
+        const unsigned keep = threshold ? mjt_keep_bits((unsigned long long)g, key, call, threshold) : 0xffu;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             float v = keep >> j & 1 ? mjt_el<TYPE>::up(in.v[j]) * scale : 0.0f;

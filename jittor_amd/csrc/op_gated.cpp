@@ -56,7 +56,7 @@ Route choose(int dtype, int64_t M, int64_t F, int64_t K, bool aligned, int* tile
     const double stages = std::ceil((double)K / 64.0);
     auto rounds = [&](double tiles, double at_once) { return std::ceil(tiles / at_once); };
     auto tiles_of = [&](int64_t rows, int64_t cols) { return (double)((M + rows - 1) / rows) * (double)((F + cols - 1) / cols); };
-    if (may("few") && M <= 16 && (forced || esz == 4 || M <= 4 || 2 * F * K * esz <= int64_t(24) << 20)) return FEW;
+    if (may("few") && M <= 16 && F < (int64_t(1) << 25) && (forced || esz == 4 || M <= 4 || 2 * F * K * esz <= int64_t(24) << 20)) return FEW;
     if (may("tiles") && esz == 2 && K >= 64 && K * 2 * 256 < (int64_t(1) << 31)) {
         const double r256 = rounds(tiles_of(256, 128), (double)cus), n128 = tiles_of(128, 64), r128 = rounds(n128, 2.0 * (double)cus);
         const double t256 = r256 * (10.0 + 1.1 * stages) * (r256 > 1 ? 1.2 : 1.0);
@@ -94,6 +94,7 @@ bool on_tiles(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tenso
     JitKernel* k = layer_kernel(name.str(), {"element.h", "gated_act.h", "gemm_dma.h"}, defs.str());
     // (as for the plain product: a build that moved registers aside behind the spelled-out reads is not run)
     if (k->spilled != 0 || k->agprs < 0 || k->agprs > tile * tile / 256) return false;
+    MJT_CHECK(tm * tn < (int64_t(1) << 23), "gated_linear: launch too large");
     jit_launch(k, (unsigned)((tm * tn + 7) / 8 * 8), 1, 256, 0,
                {bits_of_ptr(x->ptr), bits_of_ptr(w->ptr), bits_of_ptr(y ? y->ptr : nullptr), (uint64_t)M, (uint64_t)F, (uint64_t)K, (uint64_t)K, bits_of_ptr(both ? both->ptr : nullptr), 0, 0, 0, 0});
     return true;
@@ -128,20 +129,27 @@ void forward(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor
     }
     if (route == TILES && on_tiles(x, w, act, y, both, tile)) return;
     if (route != PRODUCT && gemm_gated(x->dtype, act, act_name(act), x->ptr, w->ptr, y ? y->ptr : nullptr, both ? both->ptr : nullptr, M, F, K)) return;
-    // the rest: both projections as one product in 32 bits, then the activation
-    mjt_tensor c{};
-    if (both) c = *both;
-    else {
-        const size_t bytes = (size_t)(M * 2 * F * 4);
-        if (!ctx().dry_run && !grow_kept(&g_both, &g_both_bytes, bytes)) MJT_FAIL(MJT_ERR_DEVICE, "gated_linear: no memory for gate and up");
-        c.ptr = ctx().dry_run ? (void*)(uintptr_t)0x1000 : g_both;
+    // the rest: both projections as one product in 32 bits, then the activation; where nobody wants the products, some rows at a time, so that
+    // they take 256 MB at most (or a row)
+    const int64_t most = both ? M : std::max(int64_t(1), (int64_t(256) << 20) / (2 * F * 4));
+    const int64_t rows = std::min(M, most);
+    void* mem = nullptr;
+    if (!both) {
+        if (!ctx().dry_run && !grow_kept(&g_both, &g_both_bytes, (size_t)(rows * 2 * F * 4))) MJT_FAIL(MJT_ERR_DEVICE, "gated_linear: no memory for gate and up");
+        mem = ctx().dry_run ? (void*)(uintptr_t)0x1000 : g_both;
+    }
+    for (int64_t r = 0; r < M; r += rows) {
+        mjt_tensor a = *x, c{};
+        a.shape[0] = std::min(rows, M - r);
+        a.ptr = (char*)x->ptr + r * K * dtype_size(x->dtype);
+        c.ptr = both ? both->ptr : mem;
         c.dtype = MJT_FLOAT32;
         c.ndim = 2;
-        c.shape[0] = M;
+        c.shape[0] = a.shape[0];
         c.shape[1] = 2 * F;
+        matmul_impl(&a, w, &c, 0, 1, false);
+        if (y) rows_pass(act, c.ptr, (char*)y->ptr + r * F * dtype_size(y->dtype), nullptr, y->dtype, a.shape[0], F);
     }
-    matmul_impl(x, w, &c, 0, 1, false);
-    if (y) rows_pass(act, c.ptr, y->ptr, nullptr, y->dtype, M, F);
 }
 
 void backward(const mjt_tensor* dy, const mjt_tensor* both, int act, const mjt_tensor* d) {

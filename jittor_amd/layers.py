@@ -5,6 +5,7 @@ programs use are in nn.py.  Their gradients are calls of the same kind.  Second 
 when they are asked for.
 """
 import ctypes
+import itertools
 import numbers
 
 import numpy as np
@@ -53,11 +54,11 @@ class _Generator:
         self.seed(0)
 
     def seed(self, seed):
-        self.key, self.calls = int(seed), 0
+        self.state = int(seed), itertools.count()              # (one object: threads that draw at the same time get numbers of one key)
 
     def next(self):
-        self.calls += 1
-        return self.key, self.calls - 1
+        key, calls = self.state
+        return key, next(calls)
 
 
 generator = _Generator()
@@ -82,11 +83,13 @@ def dropout(x, p, is_train, seed, offset, residual):
         residual = core._as_var(residual)
         if residual.dtype != x.dtype or list(residual.shape) != list(x.shape):
             raise ValueError("dropout: x is %s %s, the residual %s %s" % (x.dtype, list(x.shape), residual.dtype, list(residual.shape)))
+    if seed is None and offset is not None:
+        raise ValueError("dropout: an offset belongs to a seed")
     if not is_train or p == 0.0:
-        return x if residual is None else core.binary(x, residual, "add")
-    if seed is None:
-        if offset is not None:
-            raise ValueError("dropout: an offset belongs to a seed")
+        if residual is None:
+            return x
+        p, seed, offset = 0.0, 0, 0                            # (the sum alone, rounded as in training)
+    elif seed is None:
         seed, offset = generator.next()
     key = [_number(seed, "the seed"), _number(offset or 0, "the offset")]
     inputs = [x] + ([] if residual is None else [residual]) + key

@@ -59,6 +59,16 @@ def test_dropout(gpu, dtype, shape, p):
             assert np.array_equal(_got(grads[1]), ge)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_residual_is_added_without_dropout_too(gpu, dtype):
+    rng = np.random.default_rng(2)
+    (x, xe), (r, re) = _make(rng, (5, 77), dtype), _make(rng, (5, 77), dtype)
+    for y in (jt.nn.dropout(x, 0.0, True, residual=r), jt.nn.dropout(x, 0.5, False, residual=r)):
+        dx = jt.grad((y * r).sum(), x)
+        _check(_got(y), xe + re, 2 * E * (np.abs(xe) + np.abs(re)), dtype, "y")
+        assert np.array_equal(_got(dx), re)
+
+
 def test_dropout_at_the_threshold(gpu):
     """p between two multiples of 2^-16: the lower halves of the numbers decide for one element in 65536, and have to."""
     n = 1 << 17
@@ -228,6 +238,8 @@ def test_gradients_of_some_of_the_results(gpu, given):
 def test_long_heads(gpu):
     _heads("float32", (2, 3), 2, 1, 1022, 511, False, True)
     _heads("bfloat16", (2, 3), 2, 1, 1024, 512, True, True)
+    _heads("float32", (1, 2), 1, 1, 4096, 100, False, True)
+    _heads("float16", (1, 2), 1, 1, 4096, 2048, True, False)
 
 
 def test_heads_that_are_zero_or_not_finite(gpu):
@@ -469,6 +481,61 @@ def test_every_route_of_gated_projections(gpu, monkeypatch, dtype, route, shapes
             _check(_got(both), xe @ we.T, (k + 2) * E * (np.abs(xe) @ np.abs(we).T), "float32", (route, tile, rows, k, f))
             jt.sync([y])
             _check(_got(y), want, off, dtype, (route, tile, rows, k, f))
+
+
+def test_gated_in_blocks_of_rows_without_memory_for_all(gpu):
+    """An odd width goes to the plain product; gate and up of 2^25 values a block."""
+    _gated("bfloat16", 70, 33, (1 << 19) + 3, "relu")
+
+
+# ---- in graphs --------------------------------------------------------------------------------------------------------------
+def test_inputs_that_are_rebound_keep_their_value_in_what_was_built(gpu):
+    rng = np.random.default_rng(20)
+    (x, xe), (w, we), (s, se) = _make(rng, (2, 4, 4, 8), "float32"), _make(rng, (12, 8), "float32"), _make(rng, (8,), "float32", 0.1, 1.0)
+    q, k, v = jt.nn.qkv_norm_rope(x, 2, 1, s, s)
+    y = jt.nn.gated_linear(x, w)
+    dw, ds = jt.grad(y.sum(), w), jt.grad(q.sum() + v.sum(), s)
+    for u in (x, w, s):
+        u.assign(u * 3.0)
+    want, off = P.gated(xe.reshape(-1, 8), we, "silu")
+    _check(_got(y).reshape(-1, 6), want, off, "float32", "y")
+    (_, _), (dwe, dwo) = P.gated_grad(xe.reshape(-1, 8), we, "silu", np.ones((32, 6)), "float32")
+    _check(_got(dw), dwe, dwo, "float32", "dw")
+    part = xe.reshape(8, 4, 8)[:, :2]
+    _check(_got(q).reshape(8, 2, 8), P.head_norm(part, se, None, None, 1e-6, False), 64 * E * np.abs(part) * 4, "float32", "q")
+    _, dse, _, dss = P.head_norm_grad(part, se, None, None, 1e-6, False, np.ones(part.shape))
+    _check(_got(ds), dse, 128 * E * dss, "float32", "ds")
+    assert np.array_equal(_got(v).reshape(8, 1, 8), xe.reshape(8, 4, 8)[:, 3:])
+
+
+def test_profiles_name_the_calls_and_change_nothing(gpu):
+    rng = np.random.default_rng(21)
+    (x, xe), (w, we) = _make(rng, (6, 8), "float32"), _make(rng, (12, 8), "float32")
+    with jt.profile_scope() as rep:
+        y = jt.nn.gated_linear(jt.nn.dropout(x, 0.5, True, seed=1), w)
+        y.sync()
+    keep = P.kept(48, 0.5, 1, 0).reshape(6, 8)
+    want, off = P.gated(np.where(keep, 2 * xe, 0.0), we, "silu")
+    _check(_got(y), want, off, "float32", "y")
+    assert "gated_linear" in str(rep) and "dropout" in str(rep)
+
+
+@pytest.mark.parametrize("replay", [True, False])
+def test_results_of_a_call_one_after_the_other(gpu, replay):
+    """q first, then k and v: each of them once, the ones that are there already left alone."""
+    rng = np.random.default_rng(22)
+    s = jt.array(np.ones(8, np.float32))
+    with jt.flag_scope(enable_replay=replay):
+        for _ in range(4):
+            x, xe = _make(rng, (1, 4, 4, 8), "float32")
+            q, k, v = jt.nn.qkv_norm_rope(x, 2, 1, s, s)
+            q.sync()
+            at = q._device_ptr()
+            jt.sync([v, q, k])
+            assert q._device_ptr() == at
+            for o, rows in ((q, slice(0, 2)), (k, slice(2, 3))):
+                _check(_got(o)[0], P.head_norm(xe[0][:, rows], np.ones(8), None, None, 1e-6, False), 64 * E * np.abs(xe[0][:, rows]) * 4, "float32", "q or k")
+            assert np.array_equal(_got(v)[0], xe[0][:, 3:])
 
 
 # ---- all of them in one model -----------------------------------------------------------------------------------------
