@@ -218,6 +218,8 @@ bool gemm_gated(int dtype, int act, const char* act_name, const void* x, const v
 int element_type(int dtype);
 // The kernel `name` made of embedded source files behind `defines`, built once; its launcher is called for every launch, so the key is
 // all there is to look up.
+// Whether a kernel that passes over `bytes` once reads and writes past the caches (element.h).
+inline bool streams(int64_t bytes) { return bytes >= (int64_t(32) << 20); }
 JitKernel* layer_kernel(const std::string& name, std::initializer_list<const char*> files, const std::string& defines);
 
 // Threads of a workgroup of kernels/gemm_mfma.h, with float32 operands in parts or as they are.

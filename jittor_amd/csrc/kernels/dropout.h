@@ -8,7 +8,7 @@
 // for one pass in 128 (never where T's lower half is 0, p = 0.5 or 0.25): full resolution of p for half the arithmetic.
 // A dropped element is 0 whatever it held, also an infinity or NaN.
 //
-// Supplied by the host: TYPE (element type), RES, WIDE (a lane's eight elements are whole aligned vectors).
+// Supplied by the host: TYPE (element type), RES, WIDE (a lane's eight elements are whole aligned vectors), STREAMS.
 // a[0] x  a[1] residual  a[2] y  a[3] elements  a[4] key  a[5] call  a[6] T  a[7] 1 / (1 - p) (double bits)
 struct Params { void* a[8]; };
 
@@ -62,8 +62,8 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
         const int have = n - g * 8 < 8 ? (int)(n - g * 8) : 8;
         mjt_els<TYPE, 8> in, add, out;
         if (WIDE && have == 8) {
-            in = *(const mjt_els<TYPE, 8>*)(x + g * 8);
-            if (RES) add = *(const mjt_els<TYPE, 8>*)(res + g * 8);
+            in = mjt_get<TYPE, 8>(x + g * 8);
+            if (RES) add = mjt_get<TYPE, 8>(res + g * 8);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -78,7 +78,7 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
             if (RES) v += mjt_el<TYPE>::up(add.v[j]);
             out.v[j] = mjt_el<TYPE>::down(v);
         }
-        if (WIDE && have == 8) *(mjt_els<TYPE, 8>*)(y + g * 8) = out;
+        if (WIDE && have == 8) mjt_set(y + g * 8, out);
         else
 #pragma unroll
             for (int j = 0; j < 8; j++)

@@ -46,7 +46,8 @@
 // same ones, so that gate and up of a result lie in the same lane and place of two of its accumulators; the rest of the kernel
 // does not know.  On the way out gate and up go through LDS, so that a lane has VS adjacent columns of both.  p.a[2] y (GATED & 1), p.a[7] their products
 // in 32 bits, [M][2 N] (GATED & 2).  The operands' bytes for a tile are those of a plain product of 2 N columns, and neither product makes a trip to memory
-// on the way to y.
+// on the way to y.  us for 8192 x 2048 -> 5632 bfloat16: 335 (1.13 PFLOP/s), 365 with the products (past the caches; 383 to 433 through them), the plain product
+// and a pass over it 445.  The MFMAs bound it, and the results of a tile, 330 KB with the products, leave while nothing is multiplied on that compute unit.
 //
 // The MFMAs are spelled out, like the LDS reads and the waits, so that the order below is the schedule; the
 // accumulators live in the accumulation registers, which nothing but these MFMAs touches inside the loop (the
@@ -369,7 +370,6 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
     constexpr int WC = WT / 2, PITCH = WC + 8, LPR = WC / VS, IT = 32 * LPR / 64;                  // columns f of the wave; lanes a row; items a lane has of 32 rows
     static_assert(4 * 2 * 32 * PITCH * 4 <= NBUF * STAGE_BYTES, "gate and up of a wave's 32 rows in LDS");
     float* const mine = (float*)lds + wave * (2 * 32 * PITCH);
-    struct alignas(VS * 4) vec { float v[VS]; };
 #pragma unroll
     for (int i = 0; i < FR; i++) {
 #pragma unroll
@@ -381,17 +381,17 @@ extern "C" __global__ __launch_bounds__(NTHR) __attribute__((amdgpu_waves_per_eu
         for (int q = 0; q < IT; q++) {
             const int lrow = (q * 64 + lane) / LPR, lcol = (q * 64 + lane) % LPR * VS, row = m0 + wm * WT + i * 32 + lrow, col = n0 + wn * WC + lcol;
             if (row >= M || col >= N) continue;                                              // (VS divides N)
-            const vec gate = *(const vec*)&mine[lrow * PITCH + lcol], up = *(const vec*)&mine[(32 + lrow) * PITCH + lcol];
+            const mjt_els<2, VS> gate = *(const mjt_els<2, VS>*)&mine[lrow * PITCH + lcol], up = *(const mjt_els<2, VS>*)&mine[(32 + lrow) * PITCH + lcol];
             if constexpr (GATED & 2) {
                 float* both = (float*)p.a[7] + (long long)row * 2 * N + col;
-                *(vec*)both = gate;
-                *(vec*)(both + N) = up;
+                mjt_set(both, gate);
+                mjt_set(both + N, up);
             }
             if constexpr (GATED & 1) {
-                struct alignas(VS * 2) { unsigned short v[VS]; } o;
+                mjt_els<IN, VS> o;
 #pragma unroll
                 for (int k = 0; k < VS; k++) o.v[k] = mjt_el<IN>::down(mjt_activate(gate.v[k]).a * up.v[k]);
-                *(decltype(o)*)((unsigned short*)p.a[2] + (long long)row * N + col) = o;
+                mjt_set((unsigned short*)p.a[2] + (long long)row * N + col, o);
             }
         }
         mjt_wave_fence();                                                                // (before the next 32 rows overwrite these)

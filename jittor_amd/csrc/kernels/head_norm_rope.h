@@ -14,11 +14,11 @@
 // rows; a lane has V pairs of the row in each of its NC chunks, as two pieces of V adjacent elements: both halves of its pairs, so
 // turning takes no exchange.  A wave works on one token at a time, R heads of one kind in a round: cos and sin are loaded once for all heads,
 // what a round does is the same for all its lanes, and values pass without arithmetic.  IT rounds are read before the first is worked on.
-// us, floor at the rate of a large copy (5.19 TB/s): 48 heads of 128 bfloat16, 8192 tokens, heads first 41.4, 38.8, its gradient 63.3, 58.2; 48 heads of 64 float32,
-// 4096 tokens 20.8, 19.4 and 29.4, 29.1; 24 heads of 80 bfloat16 on three axes, 9477 tokens 18.0, 14.0 and 30.5, 21.0: a row of 80 keeps ten of
+// us, floor at the rate of a large copy (5.19 TB/s): 48 heads of 128 bfloat16, 8192 tokens, heads first 38.4, 38.8, its gradient 59.5, 58.2; 48 heads of 64 float32,
+// 4096 tokens 20.2, 19.4 and 27.0, 29.1; 24 heads of 80 bfloat16 on three axes, 9477 tokens 18.0, 14.0 and 30.5, 21.0: a row of 80 keeps ten of
 // sixteen lanes busy, and arithmetic bounds its gradient.
 //
-// Supplied by the host: TYPE, STYPE (types of x and of the scales), D, ROT, V, LP, NC, IT, PAIRED, FIRST, NORM, AXES, ENDS, POS (positions are
+// Supplied by the host: TYPE, STYPE (types of x and of the scales), D, ROT, V, LP, NC, IT, PAIRED, FIRST, NORM, STREAMS, AXES, ENDS, POS (positions are
 // given), BACK, SUMS (BACK with gradients of the scales).
 // a[0] x  a[1] q  a[2] k  a[3] v  (BACK: dq, dk, dv, null where missing; forward: null where not wanted)  a[4] scale of q  a[5] of k  a[6] table  a[7] positions
 // a[8] tokens  a[9] tokens of a sequence  a[10] HQ  a[11] HK  a[12] HV  a[13] eps (double bits)  a[14] positions of an axis  a[15] rows of the table
@@ -167,11 +167,11 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
 #endif
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                in0[it][c] = *(const mjt_els<TYPE, V>*)(from + first[c]);
-                in1[it][c] = *(const mjt_els<TYPE, V>*)(from + second[c]);
+                in0[it][c] = mjt_get<TYPE, V>(from + first[c]);
+                in1[it][c] = mjt_get<TYPE, V>(from + second[c]);
 #if BACK
-                g0[it][c] = *(const mjt_els<TYPE, V>*)(grad + first[c]);
-                g1[it][c] = *(const mjt_els<TYPE, V>*)(grad + second[c]);
+                g0[it][c] = mjt_get<TYPE, V>(grad + first[c]);
+                g1[it][c] = mjt_get<TYPE, V>(grad + second[c]);
 #endif
             }
         }
@@ -180,8 +180,8 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
 #pragma unroll
                 for (int c = 0; c < NC; c++)
                     if (in[c]) {
-                        *(mjt_els<TYPE, V>*)(at + first[c]) = o[c][0];
-                        *(mjt_els<TYPE, V>*)(at + second[c]) = o[c][1];
+                        mjt_set(at + first[c], o[c][0]);
+                        mjt_set(at + second[c], o[c][1]);
                     }
         };
         auto copy = [&](auto itc) {                            // a row of values, or of zeros where no gradient arrives

@@ -23,8 +23,9 @@ static void dropout_impl(const mjt_tensor* x, const mjt_tensor* residual, const 
     if (n == 0) return;
     const uintptr_t group = 8 * (uintptr_t)dtype_size(x->dtype);
     const bool wide = (uintptr_t)x->ptr % group == 0 && (uintptr_t)y->ptr % group == 0 && (!residual || (uintptr_t)residual->ptr % group == 0);
-    const std::string name = "mjt_dropout_" + std::string(mjt_dtype_name(x->dtype)) + (residual ? "_residual" : "") + (wide ? "" : "_unaligned");
-    JitKernel* k = layer_kernel(name, {"element.h", "dropout.h"}, "#define TYPE " + std::to_string(type) + "\n#define RES " + (residual ? "1" : "0") + "\n#define WIDE " + (wide ? "1" : "0") + "\n");
+    const bool far = streams(n * dtype_size(x->dtype) * (residual ? 3 : 2));
+    const std::string name = "mjt_dropout_" + std::string(mjt_dtype_name(x->dtype)) + (residual ? "_residual" : "") + (wide ? "" : "_unaligned") + (far ? "_streams" : "");
+    JitKernel* k = layer_kernel(name, {"element.h", "dropout.h"}, "#define TYPE " + std::to_string(type) + "\n#define RES " + (residual ? "1" : "0") + "\n#define WIDE " + (wide ? "1" : "0") + "\n#define STREAMS " + (far ? "1" : "0") + "\n");
     const int64_t groups = (n + 7) / 8, blocks = std::min((groups + 255) / 256, int64_t(1) << 23);
     const uint64_t threshold = (uint64_t)std::nearbyint(p * 4294967296.0);
     jit_launch(k, (unsigned)blocks, 1, 256, 0, {bits_of_ptr(x->ptr), bits_of_ptr(residual ? residual->ptr : nullptr), bits_of_ptr(y->ptr), (uint64_t)n, (uint64_t)key->ivalue,

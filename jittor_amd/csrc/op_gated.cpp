@@ -28,9 +28,10 @@ void rows_pass(int act, const void* both, const void* y, const void* d, int dtyp
     const size_t esz = (size_t)dtype_size(dtype);
     const bool wide = F % 4 == 0 && (uintptr_t)both % 16 == 0 && (uintptr_t)y % (4 * esz) == 0 && (uintptr_t)d % (4 * esz) == 0;
     const int V = wide ? 4 : 1;
-    const std::string name = std::string("mjt_gated_") + act_name(act) + (d ? "_grad_" : "_") + mjt_dtype_name(dtype) + (wide ? "" : "_single");
+    const bool far = streams(rows * F * (8 + (d ? 3 : 1) * (int64_t)esz));
+    const std::string name = std::string("mjt_gated_") + act_name(act) + (d ? "_grad_" : "_") + mjt_dtype_name(dtype) + (wide ? "" : "_single") + (far ? "_streams" : "");
     JitKernel* k = layer_kernel(name, {"element.h", "gated_act.h", "gated_rows.h"},
-                                "#define TYPE " + std::to_string(element_type(dtype)) + "\n#define V " + std::to_string(V) + "\n#define ACT " + std::to_string(act) + "\n#define BACK " + (d ? "1" : "0") + "\n");
+                                "#define TYPE " + std::to_string(element_type(dtype)) + "\n#define V " + std::to_string(V) + "\n#define ACT " + std::to_string(act) + "\n#define BACK " + (d ? "1" : "0") + "\n#define STREAMS " + (far ? "1" : "0") + "\n");
     const int64_t n = rows * F / V;
     jit_launch(k, (unsigned)std::min((n + 255) / 256, int64_t(1) << 23), 1, 256, 0, {bits_of_ptr(both), bits_of_ptr(y), bits_of_ptr(d), (uint64_t)n, (uint64_t)(F / V)});
 }
@@ -87,10 +88,11 @@ bool on_tiles(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tenso
     const int nbuf = tile == 256 ? 2 : tm * tn > cus ? 2 : 4, wpe = tile == 128 && nbuf == 2 ? 2 : 1;
     auto whole = [&](int v) { return F % v == 0 && (!y || (uintptr_t)y->ptr % (size_t)(v * 2) == 0) && (!both || (uintptr_t)both->ptr % (size_t)(v * 4) == 0); };
     const int vs = whole(4) ? 4 : whole(2) ? 2 : 1, tail = K % 64 ? 1 : 0, gated = (y ? 1 : 0) + (both ? 2 : 0);
+    const bool far = both && streams(M * F * 10);               // (y alone is what the next product reads)
     std::ostringstream name, defs;
     name << "mjt_gated_tiles_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << "_" << tile << "x" << tile << (wpe == 2 ? "_direct2" : "_direct") << (tail ? "_tail" : "") << (both ? y ? "_both" : "_products" : "");
     defs << "#define VS " << vs << "\n#define IN " << element_type(x->dtype) << "\n#define OUT 2\n#define A_KCONT 1\n#define B_KCONT 1\n#define TILE " << tile << "\n#define NBUF " << nbuf << "\n#define WPE " << wpe
-         << "\n#define GATED " << gated << "\n#define KTAIL " << tail << "\n#define ACT " << act << "\n";
+         << "\n#define GATED " << gated << "\n#define KTAIL " << tail << "\n#define ACT " << act << "\n#define STREAMS " << (far ? 1 : 0) << "\n";
     JitKernel* k = layer_kernel(name.str(), {"element.h", "gated_act.h", "gemm_dma.h"}, defs.str());
     // (as for the plain product: a build that moved registers aside behind the spelled-out reads is not run)
     if (k->spilled != 0 || k->agprs < 0 || k->agprs > tile * tile / 256) return false;

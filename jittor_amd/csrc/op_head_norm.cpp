@@ -116,12 +116,14 @@ Plan plan_for(const char* who, const mjt_tensor* x, const mjt_tensor* q_scale, c
     a.V = V;
     a.LP = LP;
     a.NC = (int)NC;
+    // (past the caches only whole lines: 8192 tokens of 48 heads of 128 bfloat16 41.8 / 38.4 us, but 9477 of 24 heads of 80 17.4 / 22.9)
+    const bool far = D * esz % 128 == 0 && streams(a.tokens * H * D * esz * (back ? 3 : 2));
     std::ostringstream defs;
-    defs << "#define TYPE " << a.type << "\n#define STYPE " << a.scale_type << "\n#define D " << D << "\n#define ROT " << rot << "\n#define V " << V << "\n#define LP " << LP << "\n#define NC " << NC
+    defs << "#define STREAMS " << (far ? 1 : 0) << "\n#define TYPE " << a.type << "\n#define STYPE " << a.scale_type << "\n#define D " << D << "\n#define ROT " << rot << "\n#define V " << V << "\n#define LP " << LP << "\n#define NC " << NC
          << "\n#define PAIRED " << (p->interleaved ? 1 : 0) << "\n#define FIRST " << (p->heads_first ? 1 : 0) << "\n#define NORM " << (q_scale ? 1 : 0) << "\n#define AXES " << axes
          << "\n#define ENDS " << ends << "\n#define POS " << (positions ? 1 : 0) << "\n";
     a.defines = defs.str();
-    a.name = std::string("mjt_head_norm_rope_") + mjt_dtype_name(x->dtype) + "_" + std::to_string(D);
+    a.name = std::string("mjt_head_norm_rope_") + mjt_dtype_name(x->dtype) + "_" + std::to_string(D) + (far ? "_streams" : "");
     auto ptr = [](const mjt_tensor* t) { return bits_of_ptr(t ? t->ptr : nullptr); };
     a.args = {ptr(x), ptr(parts[0]), ptr(parts[1]), ptr(parts[2]), ptr(q_scale), ptr(k_scale), ptr(table), ptr(positions), (uint64_t)a.tokens, (uint64_t)std::max<int64_t>(S, 1),
               (uint64_t)p->q_heads, (uint64_t)p->k_heads, (uint64_t)p->v_heads, bits_of(p->eps), (uint64_t)std::max<int64_t>(per, 1), (uint64_t)rows, 0, 0};
