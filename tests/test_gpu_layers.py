@@ -221,6 +221,14 @@ def test_many_tokens_and_heads(gpu, dtype):
     _heads(dtype, (2, 3), 70, 10, 96, 48, False, True, seed=6)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_passes_larger_than_the_caches_keep(gpu, dtype):
+    """Read and written by 32 MB and more, forward and backward: other loads and stores, the same results."""
+    _heads(dtype, (2, 1750), 16, 4, 128, 64, False, True, seed=14)
+    _heads(dtype, (2, 1801), 40, 5, 64, 32, True, True, sections=[8, 16, 8], seed=15)
+    _heads(dtype, (1, 1003), 40, 3, 192, 48, False, True, seed=16)
+
+
 def test_without_rotation_without_norm_and_with_scales_of_another_type(gpu):
     _heads("bfloat16", (2, 6), 4, 2, 64, 0, False, False)
     _heads("bfloat16", (2, 6), 4, 2, 64, 32, False, True, scaled=False)
