@@ -15,8 +15,8 @@
 // turning takes no exchange.  A wave works on one token at a time, R heads of one kind in a round: cos and sin are loaded once for all heads,
 // what a round does is the same for all its lanes, and values pass without arithmetic.  IT rounds are read before the first is worked on.
 // us, floor at the rate of a large copy (5.19 TB/s): 48 heads of 128 bfloat16, 8192 tokens, heads first 38.4, 38.8, its gradient 59.5, 58.2; 48 heads of 64 float32,
-// 4096 tokens 20.2, 19.4 and 27.0, 29.1; 24 heads of 80 bfloat16 on three axes, 9477 tokens 18.0, 14.0 and 30.5, 21.0: a row of 80 keeps ten of
-// sixteen lanes busy, and arithmetic bounds its gradient.
+// 4096 tokens 20.2, 19.4 and 27.0, 29.1; 24 heads of 80 bfloat16 on three axes, 9477 tokens 18.0, 14.0 and 30.5, 21.0 (22.5 and 31.8 in a
+// training step, whose other tensors leave less of these in the caches): a row of 80 keeps ten of sixteen lanes busy, and arithmetic bounds its gradient.
 //
 // Supplied by the host: TYPE, STYPE (types of x and of the scales), D, ROT, V, LP, NC, IT, PAIRED, FIRST, NORM, STREAMS, AXES, ENDS, POS (positions are
 // given), BACK, SUMS (BACK with gradients of the scales).
