@@ -778,6 +778,7 @@ bool backward(PyObject* loss, const std::vector<std::pair<long long, Ref>>& orde
     }
     PyObject* dt = PyModule_GetDict(g_dt);
     std::unordered_set<PyObject*> calls;                       // those whose gradients have been taken
+    std::unordered_map<PyObject*, std::vector<size_t>> results;                       // of every call, their places in `order`; filled at the first call
     for (size_t q = order.size(); q-- > 0;) {
         PyObject* v = order[q].second.p;
         auto it = grads->find(order[q].first);
@@ -810,11 +811,16 @@ bool backward(PyObject* loss, const std::vector<std::pair<long long, Ref>>& orde
             if (!calls.insert(call).second) continue;
             Ref douts(PyDict_New()), wanted(PyList_New(0));
             if (!douts || !wanted) return false;
-            for (auto& [id, u] : order) {
-                PyObject* uh = own(u.p, s__history);
-                auto found = grads->find(id);
-                if (!uh || uh == Py_None || found == grads->end() || own(PyTuple_GET_ITEM(uh, 0), s_call) != call) continue;
-                PyObject* index = own(PyTuple_GET_ITEM(uh, 0), s_index);
+            if (results.empty())
+                for (size_t r = 0; r < order.size(); r++) {
+                    PyObject* uh = own(order[r].second.p, s__history);
+                    PyObject* made = uh && uh != Py_None ? own(PyTuple_GET_ITEM(uh, 0), s_call) : nullptr;
+                    if (made) results[made].push_back(r);
+                }
+            for (size_t r : results[call]) {
+                auto found = grads->find(order[r].first);
+                if (found == grads->end()) continue;
+                PyObject* index = own(PyTuple_GET_ITEM(own(order[r].second.p, s__history), 0), s_index);
                 if (!index || PyDict_SetItem(douts.p, index, found->second.p)) return false;
             }
             for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(inputs); i++) {

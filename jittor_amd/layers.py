@@ -18,7 +18,7 @@ from .core import KernelOp, Var
 _FLOATS = ("float32", "bfloat16", "float16")
 
 
-_numbers = {}            # (name, options) -> its number
+_numbers, _next = {}, itertools.count()            # (name, options) -> its number
 
 
 class Call:
@@ -31,7 +31,11 @@ class Call:
     def key(self):
         """A number for name and options: a graph's key is worked out and looked up for every execution."""
         if self.number is None:
-            self.number = _numbers.setdefault((self.name, self.options), len(_numbers))
+            self.number = _numbers.get((self.name, self.options))
+            if self.number is None:
+                if len(_numbers) >= 4096:                      # (options that change with every step; a number is never given twice)
+                    _numbers.clear()
+                self.number = _numbers[self.name, self.options] = next(_next)
         return self.number
 
 
@@ -112,7 +116,7 @@ def _dropout_gradients(op, inputs, douts, wanted):
     dy = douts[0]
     grads = [None] * len(inputs)
     if wanted[0]:
-        grads[0] = _result(Call("dropout", p, False), 0, [dy] + list(inputs[-2:]), list(dy.shape), dy.dtype)
+        grads[0] = _result(Call("dropout", p, False), 0, [dy] + list(inputs[-2:]), list(dy.shape), dy.dtype) if p else dy
     if added and wanted[1]:
         grads[1] = dy
     return grads
@@ -203,7 +207,9 @@ def _head_norm_gradients(op, inputs, douts, wanted):
     given = tuple(i in douts for i in range(3))
     call = Call("head_norm_rope_grad", *op.call.options, given)
     ins = list(inputs) + [douts[i] for i in range(3) if given[i]]
-    scaled = op.call.options[1]
+    scaled, tabled = op.call.options[1:3]
+    if tabled and wanted[3 if scaled else 1]:
+        raise NotImplementedError("head_norm_rope: the gradient of a table of angles")
     return [_result(call, i, ins, list(u.shape), u.dtype) if want and i < (3 if scaled else 1) else None for i, (u, want) in enumerate(zip(inputs, wanted))]
 
 

@@ -243,8 +243,8 @@ def qkv_norm_rope(qkv, heads, kv_heads, q_scale=None, k_scale=None, table=None, 
     root of its mean square (plus eps) and scaled by q_scale or k_scale [dim], then turned by its position; the values as they are.
 
     `table` (rope_table) holds the angles of its first 2 * table.shape[1] elements; pairs are elements i and i + table.shape[1], or
-    neighbours with `interleaved`.  `positions` (int32 [.., tokens] or [tokens]; 0, 1, .. where left out) are rows of the table; one outside makes
-    what it turns NaN.  For images and video `sections` gives the number of pairs for each axis, and positions [axes, .., tokens].
+    neighbours with `interleaved`.  It is a constant: its gradient is refused.  `positions` (int32 [.., tokens] or [tokens]; 0, 1, .. where
+    left out) are rows of the table; one outside makes what it turns NaN.  For images and video `sections` gives the number of pairs for each axis, and positions [axes, .., tokens].
     Without scales the heads are only turned, without a table only normalised.  Results are [.., tokens, heads, dim], or with `heads_first`
     [.., heads, tokens, dim], as attention's products read them."""
     if (q_scale is None) != (k_scale is None):

@@ -112,6 +112,45 @@ def test_qkv_norm_rope_refuses(case):
                             sections=c["sections"], eps=c["eps"])
 
 
+def test_gradients_that_are_refused():
+    """Those of a table of angles, and second ones."""
+    x, table = jt.array(np.ones((1, 3, 3, 4), np.float32)), jt.nn.rope_table(8, 4)
+    q, k, v = jt.nn.qkv_norm_rope(x, 1, 1, None, None, table)
+    assert len(jt.grad((q * q).sum(), [x])) == 1
+    with pytest.raises(NotImplementedError, match="table"):
+        jt.grad((q * q).sum(), [x, table])
+    (d,) = jt.grad((q * q).sum(), [x])
+    with pytest.raises(NotImplementedError, match="second"):
+        jt.grad(d.sum(), [x])
+
+
+def test_gradient_of_the_sum_alone_is_what_arrives():
+    """Nothing is dropped with p = 0: both gradients are the one of the sum, without a launch."""
+    x, r, g = (jt.array(np.full((3, 4), v, np.float32)) for v in (1, 2, 3))
+    y = jt.nn.dropout(x, 0.0, True, residual=r)
+    dx, dr = jt.grad((y * g).sum(), [x, r])
+    assert not any(isinstance(d._op, core.KernelOp) for d in (dx, dr))
+
+
+def test_gradients_of_many_calls_in_one_graph():
+    """Every call's gradient reads the one behind it, and the results of a call are found whatever stands between them."""
+    x = y = jt.array(np.ones((2, 4), np.float32))
+    for i in range(300):
+        y = jt.nn.dropout(y * 2.0, 0.5, True, seed=1, offset=i, residual=y)
+    (d,) = jt.grad(y.sum(), [x])
+    calls, left = set(), [d]
+    seen = set()
+    while left:
+        u = left.pop()
+        if u.id in seen or u._op is None:
+            continue
+        seen.add(u.id)
+        if isinstance(u._op, core.KernelOp):
+            calls.add(u._op.call)
+        left += u._op.inputs
+    assert len(calls) == 300
+
+
 def test_gated_linear_refuses():
     for x, w, act in ((_x(3, 4), _x(5, 4), "silu"), (_x(3, 4), _x(6, 5), "silu"), (_x(3, 4), _x(6, 4), "tanh"), (_x(3, 4), _x(6, 4, dtype="float16"), "silu"), (_x(3, 4), _x(2, 3, 4), "silu"),
                       (jt.array(np.arange(12).reshape(3, 4)), jt.array(np.arange(24).reshape(6, 4)), "silu")):
