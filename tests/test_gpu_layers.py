@@ -339,6 +339,62 @@ def test_one_launch_for_three_results_and_replays(gpu):
         assert np.abs(_got(dx)[0][:, :2]).max() < 1e-3
 
 
+def _filled(gpu, shape, dtype, word):
+    """A Var whose every 32 bits are `word`, without a copy of it in host memory."""
+    v = core.Var(list(shape), dtype)
+    v._buf = core.Buffer(v.nbytes)
+    gpu.check(gpu.load().mjt_fill_u32(v._buf.ptr, word, v.nbytes // 4))
+    return v
+
+
+def test_heads_past_32_bits(gpu):
+    """Elements behind 2^32: the last tokens of [2^19 + 3, 64, 128], forward and backward."""
+    rng = np.random.default_rng(21)
+    tokens, last = (1 << 19) + 3, 4
+    x = _filled(gpu, (1, tokens, 64, 128), "float16", 0x3C003C00)
+    raw, xe = P.to_type(rng.standard_normal((last, 64, 128)), "float16")
+    gpu.h2d(x._buf.ptr + 2 * (tokens - last) * 64 * 128, raw)
+    (s, se), (t, te) = _make(rng, (128,), "float16", 0.3, 1.0), _table(rng, 40, 64)
+    at = (np.arange(tokens) % 40).astype(np.int32)
+    cos, sin = P.angles_of(te, at[None, -last:], [64], (1, last))
+    for first in (False, True):
+        q, k, v = jt.nn.qkv_norm_rope(x, 62, 1, s, s, t, jt.array(at[None]), eps=1e-5, heads_first=first)
+        dq = _filled(gpu, q.shape, "float16", 0x3C003C00)
+        (dx,) = jt.grad((q * dq).sum(), [x])
+        jt.sync([q, k, v, dx])
+        def tail(u, heads):
+            if not first:
+                return gpu.d2h(u._buf.ptr + 2 * (tokens - last) * heads * 128, [last, heads, 128], np.float16).astype(np.float64)
+            return np.stack([gpu.d2h(u._buf.ptr + 2 * ((h * tokens) + tokens - last) * 128, [last, 128], np.float16) for h in range(heads)], 1).astype(np.float64)
+        for u, rows in ((q, slice(0, 62)), (k, slice(62, 63))):
+            part = xe[:, rows]
+            z = part / np.sqrt((part * part).mean(-1, keepdims=True) + 1e-5) * se
+            _check(tail(u, part.shape[1]), P.head_norm(part, se, cos, sin, 1e-5, False), (64 + 16) * E * P.pair_size(z, cos, False), "float16", rows)
+        assert np.array_equal(tail(v, 1), xe[:, 63:])
+        want, _, off, _ = P.head_norm_grad(xe[:, :62], se, cos, sin, 1e-5, False, np.ones((last, 62, 128)))
+        got = gpu.d2h(dx._buf.ptr + 2 * (tokens - last) * 64 * 128, [last, 64, 128], np.float16).astype(np.float64)
+        _check(got[:, :62], want, (2 * 128 + 32) * E * off, "float16", "dx")
+        assert (got[:, 62:] == 0).all()
+        del q, k, v, dq, dx
+
+
+@pytest.mark.parametrize("rows", [1, 24, 300])
+def test_weights_past_32_bits(gpu, rows):
+    """2^21 + 48 rows of 2048: the last columns of both halves on each of the routes."""
+    k, f = 2048, (1 << 20) + 24
+    w = _filled(gpu, (2 * f, k), "float16", 0x3C003C00)
+    for row, value in ((f - 1, 2.0), (2 * f - 1, 3.0), (2 * f - 2, -1.0)):
+        gpu.h2d(w._buf.ptr + 2 * row * k, np.full(k, value, np.float16))
+    x = jt.array(np.full((rows, k), 1.0 / k, np.float16))
+    y = jt.nn.gated_linear(x, w, "sigmoid")
+    y.sync()
+    s = lambda g: 1.0 / (1.0 + np.exp(-g))
+    want = np.array([s(1.0)] * 6 + [-s(1.0), 3.0 * s(2.0)])
+    for row in sorted({0, rows - 1}):
+        got = gpu.d2h(y._buf.ptr + 2 * (row * f + f - 8), [8], np.float16).astype(np.float64)
+        _check(got, want, 64 * E * np.abs(want), "float16", row)
+
+
 # ---- gated projections ------------------------------------------------------------------------------------------------
 def _gated(dtype, rows, k, f, act, lead=None, seed=0):
     rng = np.random.default_rng(seed)
