@@ -12,11 +12,16 @@
 // some compute units with twice the others' work.  Four pieces at a time instead of two 38 / 13.2 / 14.0.  More than sixteen rows of x this way
 // wait for x: 24 x 2048 -> 5632 16.5, 64 x 4096 -> 11264 74; those go to tiles.
 //
-// Supplied by the host: TYPE, ACT, W, UN, BOTH (gate and up are wanted), Y (y is wanted).  Rows of x
-// and of the weights are multiples of 16 bytes and begin at one; rows past the last are read from the last, their results are not stored.
+// Supplied by the host: TYPE, ACT, W, UN, BOTH (gate and up are wanted), Y (y is wanted), RAGGED (otherwise rows of x
+// and of the weights are multiples of 16 bytes and begin at one).  Rows past the last are read from the last, their results are not stored.
 // a[0] x  a[1] weights  a[2] y  a[3] both  a[4] M  a[5] F  a[6] K
 struct Params { void* a[7]; };
 typedef unsigned mjt_piece __attribute__((ext_vector_type(4)));
+#if RAGGED
+typedef unsigned mjt_there __attribute__((ext_vector_type(4), aligned(sizeof(typename mjt_el<TYPE>::raw))));      // a piece in memory
+#else
+typedef mjt_piece mjt_there;
+#endif
 typedef float mjt_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 mjt_b16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 mjt_h16x8 __attribute__((ext_vector_type(8)));
@@ -49,17 +54,24 @@ extern "C" __global__ __launch_bounds__(W * 64) void ENTRY(Params p) {
         mjt_piece a[UN], b[UN];
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            a[u] = __builtin_nontemporal_load((const mjt_piece*)(w + k + u * STEP));
-            b[u] = *(const mjt_piece*)(x + k + u * STEP);
+            a[u] = __builtin_nontemporal_load((const mjt_there*)(w + k + u * STEP));
+            b[u] = *(const mjt_there*)(x + k + u * STEP);
         }
 #pragma unroll
         for (int u = 0; u < UN; u++) acc = mjt_multiply(a[u], b[u], acc);
     }
     // the last run of the row ends with one of the waves: piece by piece, nothing past K
     for (int end = k + UN * STEP; k < end && k < K; k += STEP) {
-        const bool in = k + at < K;
-        const mjt_piece none = {0, 0, 0, 0};
-        acc = mjt_multiply(in ? *(const mjt_piece*)(w + k) : none, in ? *(const mjt_piece*)(x + k) : none, acc);
+        const int have = K - k - at;                           // elements that the lane's piece has
+        mjt_piece a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+        if (have >= EPL) a = *(const mjt_there*)(w + k), b = *(const mjt_there*)(x + k);
+#if RAGGED
+        else
+#pragma unroll
+            for (int j = 0; j < EPL; j++)
+                if (j < have) ((raw*)&a)[j] = w[k + j], ((raw*)&b)[j] = x[k + j];
+#endif
+        acc = mjt_multiply(a, b, acc);
     }
     // D of a 16 x 16 tile: lane holds column lane % 16 (a row of x), rows 4 * (lane / 16) + e (g, then u)
     __shared__ float part[W][16][20];

@@ -65,6 +65,10 @@
 // results are not stored); k beyond K is zeroed in both operands.  Leading dimensions are
 // multiples of 16 bytes and the operand pointers 16-byte aligned (the host sends
 // everything else to the plain kernel below).
+//
+// RAGGED 1: rows of any length that begin anywhere (at an element); loads of 16 bytes need no alignment here.  A chunk that a row's end cuts is
+// loaded element by element in the last stage of a sum; of an operand with m or n innermost, which has at least EPC columns, the last
+// EPC columns are loaded instead and go to their own places, where the chunk before writes the same.
 
 #if IN == 2
 typedef float TIN;
@@ -100,6 +104,9 @@ typedef unsigned short TIN;
 #ifndef GATED
 #define GATED 0
 #endif
+#ifndef RAGGED
+#define RAGGED 0
+#endif
 #ifndef SLICED
 #define SLICED 0                 // 1: workgroup (tile, slice) sums stages slice * a[9] .. of K into its own float32 C (or y), a[11] apart
 #endif
@@ -119,6 +126,11 @@ typedef unsigned short TIN;
 
 typedef float mjt_f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned mjt_u32x4v __attribute__((ext_vector_type(4)));
+#if RAGGED
+typedef unsigned mjt_u32x4m __attribute__((ext_vector_type(4), aligned(16 / EPC)));    // in memory
+#else
+typedef mjt_u32x4v mjt_u32x4m;
+#endif
 #if IN == 0
 typedef __bf16 mjt_h8 __attribute__((ext_vector_type(8)));
 #define MJT_MFMA16(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0)
@@ -216,6 +228,9 @@ template <int I, int N, class F> __device__ __forceinline__ void mjt_static_for(
 template <int ROWS, bool KCONT, bool HALVES = false> struct mjt_stager {       // HALVES: the tile's rows are ROWS / 2 of rmax rows and the same of the rmax rows behind them
     static constexpr int PER = ROWS * KC / NTHR;          // 16-byte moves per thread
     mjt_u32x4v reg[PER];
+#if RAGGED
+    int first, rows;                                      // of the tile, of the operand
+#endif
 
     template <int I, bool FULL> __device__ __forceinline__ void fetch(const TIN* __restrict__ p, long long ld, int r0, int rmax, int k0, int K, int tid) {
         if constexpr (KCONT) {
@@ -225,8 +240,23 @@ template <int ROWS, bool KCONT, bool HALVES = false> struct mjt_stager {       /
             row = row < rmax ? row : rmax - 1;
             if (HALVES && c / KC >= ROWS / 2) row += rmax;
             const int k = k0 + (c % KC) * EPC;
+#if RAGGED
+            if constexpr (!FULL) {
+                if (k + EPC > K) {                        // element by element; what is past the end is zeroed in commit
+                    const TIN* q = p + (long long)row * ld;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#if IN == 2
+                        reg[I][j] = __float_as_uint(q[k + j < K ? k + j : K - 1]);
+#else
+                        reg[I][j] = (unsigned)q[k + 2 * j < K ? k + 2 * j : K - 1] | (unsigned)q[k + 2 * j + 1 < K ? k + 2 * j + 1 : K - 1] << 16;
+#endif
+                    return;
+                }
+            }
+#endif
             const int kk = FULL || k < K ? k : 0;         // a chunk past the end reads chunk 0 and is zeroed in commit
-            reg[I] = *(const mjt_u32x4v*)(p + (long long)row * ld + kk);
+            reg[I] = *(const mjt_u32x4m*)(p + (long long)row * ld + kk);
         } else {
             // blocks of EPC k-rows x EPC columns: EPC lanes each load 16 bytes (EPC columns) of one k-row.
             // Block b = tid / EPC + I * (NTHR / EPC): column group b % (ROWS / EPC), k-chunk b / (ROWS / EPC);
@@ -234,10 +264,16 @@ template <int ROWS, bool KCONT, bool HALVES = false> struct mjt_stager {       /
             const int b = tid / EPC + I * (NTHR / EPC);
             const int cg = b % (ROWS / EPC), kc = b / (ROWS / EPC);
             int col = r0 + cg * EPC;
+#if RAGGED
+            first = r0;
+            rows = rmax;
+            col = col + EPC <= rmax ? col : rmax - EPC;             // a group that the operand's end cuts, or outside, reads the last EPC columns
+#else
             col = col < rmax ? col : ((rmax - 1) / EPC) * EPC;      // a group outside the operand reads the last one (ld is a multiple of EPC: a group never leaves its row)
+#endif
             const int k = k0 + kc * EPC + tid % EPC;
             const int kk = FULL || k < K ? k : 0;
-            reg[I] = *(const mjt_u32x4v*)(p + (long long)kk * ld + col);
+            reg[I] = *(const mjt_u32x4m*)(p + (long long)kk * ld + col);
         }
     }
     template <int I, bool FULL, bool SP> __device__ __forceinline__ void commit(unsigned char* lds, int k0, int K, int tid) const {
@@ -268,6 +304,13 @@ template <int ROWS, bool KCONT, bool HALVES = false> struct mjt_stager {       /
             v = mjt_transpose4x4_b32(v, tid);
 #else
             v = mjt_transpose8x8_b16(v, tid);
+#endif
+#if RAGGED
+            const int group = row - tid % EPC, cut = first + group + EPC - rows;       // columns of the group that the operand does not have
+            if (cut > 0) {
+                if (cut >= EPC || row < cut) return;      // (those places stay zero; the last columns may begin in front of the tile)
+                row -= cut;
+            }
 #endif
         }
         mjt_put<SP>(lds, row, kc, v);
@@ -521,6 +564,10 @@ extern "C" __global__ __launch_bounds__(NTHR) void ENTRY(Params p) {
 #endif
     // NBUF 1: the host promises K <= KS, a single stage -- one staging buffer, so twice as many workgroups fit a compute unit
     __shared__ __attribute__((aligned(16))) unsigned char lds[NBUF][(TM + TN) * SPLIT_ROWB];
+#if RAGGED && !(A_KCONT && B_KCONT)
+    for (int i = threadIdx.x; i < (int)sizeof(lds) / 16; i += NTHR) ((mjt_u32x4v*)&lds[0][0])[i] = (mjt_u32x4v)(0u);      // (places that no column has)
+    __syncthreads();
+#endif
 #if SPLIT
     __shared__ int in_float32;                                 // some sum is not finite
     if (threadIdx.x == 0) in_float32 = 0;

@@ -39,9 +39,12 @@ void rows_pass(int act, const void* both, const void* y, const void* d, int dtyp
 // The ways to run the projections, by estimated time.
 //   FEW (kernels/gated_few.h): up to 16 rows.  16-bit operands of more than 4 rows and 24 MB of weights are better off on tiles, which load x once
 //   for 32 columns (us few / MFMA: 16 x 1024 -> 2816 6.4 / 7.4; 16 x 2048 -> 5632 14.7 / 10.8, of 4 rows 11.9 / 11.1); float32 MFMAs are slower
-//   than the loads of x (float32 16 x 2048 -> 5632 28 / 33).
+//   than the loads of x (float32 16 x 2048 -> 5632 28 / 33).  Rows that are no whole 16-byte pieces: up to 20 MB, as their loads cross lines (us few / MFMA or PRODUCT:
+//   bfloat16 1 x 1501 -> 1500 6.3 / 9.8, of 16 rows 9.2 / 12.8, 1 x 2231 -> 2610 14.6 / 13.3, of 16 26.1 / 17.8; float32 4 x 1501 -> 1500 8.4 / 12.8, 4 x 2231 -> 2610 22.3 / 19.5).
 //   TILES (kernels/gemm_dma.h): 16-bit operands on 256 x 256 tiles, one to a compute unit, or 128 x 128, two to a unit.
-//   MFMA (kernels/gemm_mfma.h): any type; a product that is better cut into slices of its sum goes to PRODUCT, the plain product in 32 bits and a pass over it.
+//   MFMA (kernels/gemm_mfma.h): any type and rows of any length; a product that is better cut into slices of its sum goes to PRODUCT, the plain product in
+//   32 bits and a pass over it (before rows of any length ran here, us then / now: bfloat16 36 x 46 -> 256 23 / 5.7, 777 x 1001 -> 2600 42.1 / 32.8, 4000 x 45 -> 3001 67.7 / 30.7;
+//   float32 3722 x 99 -> 3968 135 / 101, 1024 x 513 -> 1377 45.5 / 30.2).
 // A stage of 64 elements of the sum takes 1.1 us on a 256 x 256 tile, 0.33 on a 128 x 128 tile with a unit to itself and 0.66 for two of them (more
 // where the sum is long and neighbours drift apart), 0.25 on a 64 x 64 tile; a round begins with the first loads and ends with the
 // activations and stores, 10, 6 and 3.5 us.  Rows that are no whole 128-byte lines cost a quarter more.
@@ -53,12 +56,13 @@ Route choose(int dtype, int64_t M, int64_t F, int64_t K, bool aligned, int* tile
     const int64_t esz = dtype_size(dtype), cus = ctx().dry_run || ctx().prop.multiProcessorCount <= 0 ? 256 : ctx().prop.multiProcessorCount;
     const char* forced = getenv("MJT_GATED");                  // (a switch for measurements and tests; a route that does not cover the call is left out all the same)
     auto may = [&](const char* name) { return !forced || !strcmp(forced, name); };
-    if (!aligned || K == 0) return PRODUCT;
+    if (K == 0) return PRODUCT;
+    const int64_t bytes = 2 * F * K * esz;
     const double stages = std::ceil((double)K / 64.0);
     auto rounds = [&](double tiles, double at_once) { return std::ceil(tiles / at_once); };
     auto tiles_of = [&](int64_t rows, int64_t cols) { return (double)((M + rows - 1) / rows) * (double)((F + cols - 1) / cols); };
-    if (may("few") && M <= 16 && F < (int64_t(1) << 25) && (forced || esz == 4 || M <= 4 || 2 * F * K * esz <= int64_t(24) << 20)) return FEW;
-    if (may("tiles") && esz == 2 && K >= 64 && K * 2 * 256 < (int64_t(1) << 31)) {
+    if (may("few") && M <= 16 && F < (int64_t(1) << 25) && (forced || (aligned ? esz == 4 || M <= 4 || bytes <= int64_t(24) << 20 : bytes <= int64_t(20) << 20))) return FEW;
+    if (may("tiles") && aligned && esz == 2 && K >= 64 && K * 2 * 256 < (int64_t(1) << 31)) {
         const double r256 = rounds(tiles_of(256, 128), (double)cus), n128 = tiles_of(128, 64), r128 = rounds(n128, 2.0 * (double)cus);
         const double t256 = r256 * (10.0 + 1.1 * stages) * (r256 > 1 ? 1.2 : 1.0);
         const double t128 = n128 <= (double)cus ? 5.3 + 0.335 * stages : r128 * (6.0 + 0.66 * stages * (1.0 + std::max(0.0, stages - 32.0) / 64.0)) * (r128 > 1 && stages >= 32.0 ? 1.2 : 1.0);
@@ -73,9 +77,10 @@ Route choose(int dtype, int64_t M, int64_t F, int64_t K, bool aligned, int* tile
 void few_rows(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
     const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2;
     const int W = 8, UN = 2;
+    const bool ragged = K * dtype_size(x->dtype) % 16 != 0 || (uintptr_t)x->ptr % 16 != 0 || (uintptr_t)w->ptr % 16 != 0;
     std::ostringstream name, defs;
-    name << "mjt_gated_few_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << (both ? y ? "_both" : "_products" : "");
-    defs << "#define TYPE " << element_type(x->dtype) << "\n#define ACT " << act << "\n#define W " << W << "\n#define UN " << UN << "\n#define BOTH " << (both ? 1 : 0) << "\n#define Y " << (y ? 1 : 0) << "\n";
+    name << "mjt_gated_few_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << (ragged ? "_ragged" : "") << (both ? y ? "_both" : "_products" : "");
+    defs << "#define RAGGED " << (ragged ? 1 : 0) << "\n#define TYPE " << element_type(x->dtype) << "\n#define ACT " << act << "\n#define W " << W << "\n#define UN " << UN << "\n#define BOTH " << (both ? 1 : 0) << "\n#define Y " << (y ? 1 : 0) << "\n";
     JitKernel* k = layer_kernel(name.str(), {"element.h", "gated_act.h", "gated_few.h"}, defs.str());
     jit_launch(k, (unsigned)((F + 7) / 8), 1, W * 64, 0,
                {bits_of_ptr(x->ptr), bits_of_ptr(w->ptr), bits_of_ptr(y ? y->ptr : nullptr), bits_of_ptr(both ? both->ptr : nullptr), (uint64_t)M, (uint64_t)F, (uint64_t)K});
@@ -149,7 +154,10 @@ void forward(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor
         c.ndim = 2;
         c.shape[0] = a.shape[0];
         c.shape[1] = 2 * F;
-        matmul_impl(&a, w, &c, 0, 1, false);
+        {
+            Nearest nearest;                                   // (which takes rows of any length as they lie)
+            matmul_impl(&a, w, &c, 0, 1, false);
+        }
         if (y) rows_pass(act, c.ptr, (char*)y->ptr + r * F * dtype_size(y->dtype), nullptr, y->dtype, a.shape[0], F);
     }
 }

@@ -112,7 +112,7 @@ static TileChoice choose_tiles(int in_dtype, int64_t M, int64_t N, int64_t K, in
     const int64_t ks = esz == 2 ? 64 : 32, stages = (K + ks - 1) / ks;
     int64_t slices = 1, per = stages;
     bool split = false;
-    const bool sliceable = batch == 1 && !tile_m && !tile_n && ldc == N;
+    const bool sliceable = batch == 1 && !tile_m && !tile_n && ldc == N;          // (the slices' results are folded as whole rows)
     const double tiles64 = (double)((M + 63) / 64) * ((N + 63) / 64) * batch;
     auto crowd = [&](double wgs) { const double r = std::ceil(wgs / cus); return 1.0 + 0.8 * (r - 1.0); };
     const double st = esz == 2 ? 0.5 : 0.75;
@@ -144,6 +144,12 @@ static TileChoice choose_tiles(int in_dtype, int64_t M, int64_t N, int64_t K, in
     return {best_mi, best_ni, slices, per, stages, split};
 }
 
+// Whether a product with rows that are no whole 16-byte pieces runs on the general kernel as it lies: those of the layers' operators, whose
+// operands have k innermost or a piece's worth of columns.  (Others keep the kernels, and so the sums, that they had.)
+static bool lies_ragged(int dtype, int64_t batch, bool a_wide, bool b_wide) {
+    return Nearest::on() && batch == 1 && (dtype == MJT_BFLOAT16 || dtype == MJT_FLOAT16 || dtype == MJT_FLOAT32) && a_wide && b_wide && !getenv("MJT_GEMM_PLAIN");
+}
+
 // One strided-batched product C[b] = A'[b] * B'[b] over plain pointers: M x K times K x N, leading dimensions and
 // batch strides in elements (a batch stride of 0 shares the operand).  a_kcont / b_kcont: the operand's memory has
 // k innermost (a as given, b transposed).
@@ -159,6 +165,9 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
     };
     const bool fast = mfma_type && out_ok && !getenv("MJT_GEMM_PLAIN") && al16(A, lda, sa) && al16(B, ldb, sb) &&
                       M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31) && batch < 65536;
+    const int64_t epc = 16 / esz;
+    const bool ragged = !fast && out_ok && !tile_m && !tile_n && lies_ragged(in_dtype, batch, a_kcont || M >= epc, b_kcont || N >= epc) &&
+                        M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31);
     std::vector<uint64_t> args{bits_of_ptr(A), bits_of_ptr(B), bits_of_ptr(C), (uint64_t)M, (uint64_t)N, (uint64_t)K,
                                (uint64_t)lda, (uint64_t)ldb, (uint64_t)ldc, (uint64_t)sa, (uint64_t)sb, (uint64_t)sc};
     // 256 x 256 tiles that fill some rounds of the compute units and less than 0.7 of another: the whole rounds' tile rows first, and
@@ -242,7 +251,7 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
             if (ep.on) check_no_epilogue();                      // (the product without the group is the better one)
         }
     }
-    if (fast) {
+    if (fast || ragged) {
         const TileChoice chosen = choose_tiles(in_dtype, M, N, K, batch, a_kcont, b_kcont, tile_m, tile_n, ldc);
         const int best_mi = chosen.mi, best_ni = chosen.ni;
         int64_t slices = chosen.slices;
@@ -256,14 +265,14 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
         const bool one_stage = stages == 1 && !getenv("MJT_GEMM_TWO_BUFFERS");       // a single stage of the kernel's k loop
         const EpilogueCode ep = epilogue_code(1, 12, out_dtype, slices == 1 && ldc == N && (batch == 1 || sc == M * N) ? M * N * batch : -1);
         std::ostringstream key;
-        key << "gemm|" << in << out << MI << NI << a_kcont << b_kcont << one_stage << (slices > 1) << split << ep.key;
+        key << "gemm|" << in << out << MI << NI << a_kcont << b_kcont << one_stage << (slices > 1) << split << ragged << ep.key;
         JitKernel* k = cached(key.str());
         if (!k) {
             std::ostringstream name;
             name << "mjt_gemm_mfma_" << mjt_dtype_name(in_dtype) << "_" << (out == 2 ? "float32" : mjt_dtype_name(out_dtype)) << "_" << 64 * MI << "x" << 64 * NI
-                 << (a_kcont ? "_n" : "_t") << (b_kcont ? "t" : "n") << (one_stage ? "_k1" : "") << (split ? "_parts" : "") << (slices > 1 ? "_slices" : "") << (out == 3 ? "_nearest" : "") << ep.suffix();
+                 << (a_kcont ? "_n" : "_t") << (b_kcont ? "t" : "n") << (one_stage ? "_k1" : "") << (split ? "_parts" : "") << (slices > 1 ? "_slices" : "") << (ragged ? "_ragged" : "") << (out == 3 ? "_nearest" : "") << ep.suffix();
             std::ostringstream src;
-            src << ep.defs << "#define NBUF " << (one_stage ? 1 : 2) << "\n#define SLICED " << (slices > 1 ? 1 : 0) << "\n#define SPLIT " << (split ? 1 : 0) << "\n";
+            src << ep.defs << "#define RAGGED " << (ragged ? 1 : 0) << "\n#define NBUF " << (one_stage ? 1 : 2) << "\n#define SLICED " << (slices > 1 ? 1 : 0) << "\n#define SPLIT " << (split ? 1 : 0) << "\n";
             src << "#define ENTRY " << name.str() << "\n#define IN " << in << "\n#define OUT " << out << "\n#define MI " << MI
                 << "\n#define NI " << NI << "\n#define A_KCONT " << (a_kcont ? 1 : 0) << "\n#define B_KCONT " << (b_kcont ? 1 : 0) << "\n";
             if (split) src << embedded_source("split.h") << "\n";
@@ -315,15 +324,20 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
 bool gemm_gated(int dtype, int act, const char* act_name, const void* x, const void* w, void* y, void* both, int64_t M, int64_t F, int64_t K) {
     const int esz = dtype_size(dtype);
     TileChoice t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 2 * F);
+    // A sum in slices needs the plain product, a launch that adds them up and one for the activation; of 16-bit operands it is worth that from 48
+    // stages on (us in slices / whole: bfloat16 24 x 2048 -> 261 12.6 / 10.3, 252 x 2584 -> 896 15.2 / 12.4, 600 x 3000 -> 300 17.2 / 14.1, on the other side 1247 x 3952
+    // -> 56 12.1 / 15.7, 130 x 4096 -> 130 10.3 / 16.7; float32 103 x 1584 -> 50 11.0 / 29.6).
+    if (t.slices > 1 && esz == 2 && t.stages < 48) t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 0);
     if (t.slices > 1) return false;
     t.mi = std::min(t.mi, 2);                                   // (a tile's results have to fit its LDS)
     t.ni = std::min(t.ni, 2);
     const int in = dtype == MJT_BFLOAT16 ? 0 : dtype == MJT_FLOAT16 ? 1 : 2, gated = (y ? 1 : 0) + (both ? 2 : 0);
     const bool one_stage = t.stages == 1 && t.mi * t.ni == 1;
     const int vs = F % 4 == 0 && (uintptr_t)y % (size_t)(4 * esz) == 0 && (uintptr_t)both % 16 == 0 ? 4 : 1;
+    const bool ragged = K * esz % 16 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0;
     std::ostringstream name, defs;
-    name << "mjt_gated_mfma_" << act_name << "_" << mjt_dtype_name(dtype) << "_" << 64 * t.mi << "x" << 64 * t.ni << (one_stage ? "_k1" : "") << (t.split ? "_parts" : "") << (both ? y ? "_both" : "_products" : "");
-    defs << "#define NBUF " << (one_stage ? 1 : 2) << "\n#define SPLIT " << (t.split ? 1 : 0) << "\n#define IN " << in << "\n#define OUT 2\n#define MI " << t.mi << "\n#define NI " << t.ni
+    name << "mjt_gated_mfma_" << act_name << "_" << mjt_dtype_name(dtype) << "_" << 64 * t.mi << "x" << 64 * t.ni << (one_stage ? "_k1" : "") << (t.split ? "_parts" : "") << (ragged ? "_ragged" : "") << (both ? y ? "_both" : "_products" : "");
+    defs << "#define RAGGED " << (ragged ? 1 : 0) << "\n#define NBUF " << (one_stage ? 1 : 2) << "\n#define SPLIT " << (t.split ? 1 : 0) << "\n#define IN " << in << "\n#define OUT 2\n#define MI " << t.mi << "\n#define NI " << t.ni
          << "\n#define A_KCONT 1\n#define B_KCONT 1\n#define GATED " << gated << "\n#define VS " << vs << "\n#define ACT " << act << "\n";
     JitKernel* k = t.split ? layer_kernel(name.str(), {"element.h", "gated_act.h", "split.h", "gemm_mfma.h"}, defs.str()) : layer_kernel(name.str(), {"element.h", "gated_act.h", "gemm_mfma.h"}, defs.str());
     const int64_t tiles = ((M + 64 * t.mi - 1) / (64 * t.mi)) * ((F + 32 * t.ni - 1) / (32 * t.ni)), grid = (tiles + 7) / 8 * 8;
@@ -447,8 +461,13 @@ void matmul_impl(const mjt_tensor* a, const mjt_tensor* b, const mjt_tensor* c, 
         const double rounds = std::max(1.0, 0.5 + (double)(batch * ((n + 63) / 64) * ((k + 63) / 64)) / (double)(2 * units));
         const double copied = (double)((pad_a ? ra * lap : 0) + (pad_b ? rb * lbp : 0)) * (esz == 2 ? 2.2e-6 : 4e-6);
         const bool pays = batch == 1 || ((m >= 48 || copies == 1) && copied <= 0.09 * (double)m * rounds - (esz == 2 ? 5.0 : 3.5) + (copies == 1 ? 2.5 : 0.0));
-        if ((pad_a || pad_b) && a->dtype != MJT_FLOAT64 && !share_a && batch < 65536 && !getenv("MJT_GEMM_PLAIN") && !getenv("MJT_NO_FASTPATH") &&
-            worth((double)batch * n * k * m) && pays && (!pad_a || ra * lap * esz <= most) && (!pad_b || rb * lbp * esz <= most)) {
+        // Products that take rows of any length as they lie (gemm_launch): float32 always, 16 bits until a copy's aligned loads give back what it
+        // takes (us copied / as they lie: bfloat16, one copy, 64 x 10000 x 1001 24.1 / 14.5, 1000 x 1400 x 1001 18.0 / 17.3, on the other side 777 x 5200 x 1001 42.4 /
+        // 51.6; both, 2000 x 2002 x 1001 37.3 / 33.2, on the other side 4000 x 6002 x 1999 172 / 202; float32 1024 x 2754 x 513 44.7 / 35.1, 4000 x 6002 x 999 381 / 351).
+        const double macs = (double)batch * n * k * m;
+        const bool as_they_lie = lies_ragged(a->dtype, batch, !trans_a || n >= epc, trans_b || k >= epc) && (esz == 4 || macs < (copies == 1 ? 1.5e9 : 1e10));
+        if ((pad_a || pad_b) && !as_they_lie && a->dtype != MJT_FLOAT64 && !share_a && batch < 65536 && !getenv("MJT_GEMM_PLAIN") && !getenv("MJT_NO_FASTPATH") &&
+            worth(macs) && pays && (!pad_a || ra * lap * esz <= most) && (!pad_b || rb * lbp * esz <= most)) {
             const void* pa = pad_a ? padded_rows(0, a->ptr, a->dtype, ra, lda, lap) : a->ptr;
             const void* pb = !pad_b ? b->ptr : pa ? padded_rows(1, b->ptr, b->dtype, rb, ldb, lbp) : nullptr;
             const int64_t la = pad_a ? lap : lda, lb = pad_b ? lbp : ldb;

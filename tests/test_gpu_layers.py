@@ -552,6 +552,36 @@ def test_gated_in_blocks_of_rows_without_memory_for_all(gpu):
     _gated("bfloat16", 70, 33, (1 << 19) + 3, "relu")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ta,tb", [(0, 0), (1, 0), (0, 1)])
+@pytest.mark.parametrize("m,n,k", [(70, 9, 65), (9, 70, 400), (8, 8, 33), (5, 300, 77), (300, 7, 129), (129, 131, 127), (257, 385, 1001), (1, 1, 1), (3, 2, 9), (64, 71, 4099), (700, 1030, 61)])
+def test_products_of_rows_of_any_length(gpu, dtype, ta, tb, m, n, k):
+    """Operands whose rows are no whole 16-byte pieces, as they lie where they have k innermost or a piece of columns; an infinity behind the
+    last element of each is no part of it."""
+    import ctypes
+    rng = np.random.default_rng(m + n + k)
+    raws = [P.to_type(rng.standard_normal(shape), dtype) for shape in ((k, m) if ta else (m, k), (n, k) if tb else (k, n))]
+    whole = [jt.from_storage(np.concatenate([raw.reshape(-1), np.full(64, P.to_type(np.array(np.inf), dtype)[0])]), dtype) for raw, _ in raws]
+    whole.append(jt.from_storage(np.full(m * n + 64, P.to_type(np.array(7.0), dtype)[0]), dtype))
+    pointers = [v.raw_ptr() for v in whole]
+    t = [gpu.tensor(p, dtype, shape) for p, shape in zip(pointers, [raws[0][0].shape, raws[1][0].shape, (m, n)])]
+    gpu.check(gpu.load().mjt_matmul_nearest(*[ctypes.byref(u) for u in t], ta, tb))
+    wide = 4 if dtype == "float32" else 8
+    if ((m if ta else k) % wide or (k if tb else n) % wide) and (ta == 0 or m >= wide) and (tb == 1 or n >= wide):
+        assert "_ragged" in gpu.last_kernel()
+    a, b = raws[0][1].T if ta else raws[0][1], raws[1][1].T if tb else raws[1][1]
+    got = gpu.d2h(pointers[2], [m * n + 64], raws[0][0].dtype)               # (the Var still has what it was made from)
+    got = (bf16_bits_to_f32(got) if dtype == "bfloat16" else got).astype(np.float64)
+    _check(got[:m * n].reshape(m, n), a @ b, (k + 2) * E * (np.abs(a) @ np.abs(b)), dtype, (ta, tb))
+    assert (got[m * n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,f", [(2, 95, 40), (16, 1003, 24), (36, 46, 256), (24, 2231, 40), (90, 4099, 33), (600, 99, 500), (260, 515, 1030)])
+def test_gated_rows_of_any_length(gpu, dtype, rows, k, f):
+    _gated(dtype, rows, k, f, "silu", seed=rows + k)
+
+
 # ---- in graphs --------------------------------------------------------------------------------------------------------------
 def test_inputs_that_are_rebound_keep_their_value_in_what_was_built(gpu):
     rng = np.random.default_rng(20)
