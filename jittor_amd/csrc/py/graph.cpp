@@ -39,7 +39,7 @@ struct Ref {
 PyObject* keep(PyObject* p) { Py_XINCREF(p); return p; }
 
 #define NAMES(X) X(shape) X(num) X(dtype) X(_op) X(_history) X(id) X(_out_ref) X(inputs) X(amp) X(op) X(bcast_mask) X(keepdims_mask) X(reduce_mask) X(is_scalar) \
-    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) X(call) X(index) X(_device_ptr) X(int64) X(int32) \
+    X(_consumers) X(_compile_options) X(compile_options) X(amp_reg) X(_buf) X(_host) X(_stop_fuse) X(indexes) X(overflow_value) X(overflow_conditions) X(same_memory) X(sig) X(call) X(index) X(number) X(key) X(_device_ptr) X(int64) X(int32) \
     X(_binary_dtypes) X(binary_dtype_infer) X(unary_dtype_infer) X(reduce_dtype_infer) X(dtype_infer) X(cast) X(add) X(mean) X(float16) X(bfloat16) X(float32)
 #define DECLARE(n) PyObject* s_##n;
 NAMES(DECLARE)
@@ -648,11 +648,8 @@ bool in_set(PyObject* set, PyObject* v) {
     return i && PySet_Contains(set, i) == 1;
 }
 bool is_text(PyObject* s, const char* t) { return s && PyUnicode_Check(s) && PyUnicode_CompareWithASCIIString(s, t) == 0; }
-// A Var of its own with the value of a number's shared one: what array(number, dtype) makes, without converting the number again.
-PyObject* own_number(PyObject* shared) {
-    PyObject* host = own(shared, s__host);
-    PyObject* dtype = own(shared, s_dtype);
-    if (!host || host == Py_None || !dtype) { PyErr_SetString(PyExc_RuntimeError, "a number without its value"); return nullptr; }
+// A Var of one element whose value is in host memory, a number.
+PyObject* number_of(PyObject* host, PyObject* dtype) {
     PyObject* d;
     Ref v(instance(t_var, &d));
     if (!v || !put(d, s_shape, Py_BuildValue("[i]", 1)) || !put(d, s_num, PyLong_FromLong(1)) || PyDict_SetItem(d, s_dtype, dtype) || PyDict_SetItem(d, s__op, Py_None) ||
@@ -661,6 +658,18 @@ PyObject* own_number(PyObject* shared) {
     PyObject* co = PyDict_GetItemWithError(g_flags, s_compile_options);
     if (co && PyObject_IsTrue(co) == 1 && !put(d, s__compile_options, PyObject_CallOneArg((PyObject*)&PyDict_Type, co))) return nullptr;
     return v.give();
+}
+// A Var of its own with the value of a number's shared one: what array(number, dtype) makes, without converting the number again.
+PyObject* own_number(PyObject* shared) {
+    PyObject* host = own(shared, s__host);
+    PyObject* dtype = own(shared, s_dtype);
+    if (!host || host == Py_None || !dtype) { PyErr_SetString(PyExc_RuntimeError, "a number without its value"); return nullptr; }
+    return number_of(host, dtype);
+}
+// number_var(host, dtype): such a Var from an array of one element, which it keeps
+PyObject* py_number_var(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 2 || !PyUnicode_Check(args[1])) return PyErr_Format(PyExc_TypeError, "number_var(host, dtype)");
+    return number_of(args[0], args[1]);
 }
 PyObject* number_like(double value, bool whole, PyObject* like) {
     Shape s;
@@ -1063,7 +1072,13 @@ PyObject* py_signature(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             k.b.push_back(flag(op, s_same_memory) ? 1 : 0);
             ok = !PyErr_Occurred() && k.texts(get(s_indexes)) && k.texts(get(s_overflow_conditions));
         } else if (t == t_reindex_reduce) { k.b.push_back('s'); ok = k.text(get(s_op)) && k.texts(get(s_indexes)) && k.texts(get(s_overflow_conditions)); }
-        else {
+        else if (PyObject* call = get(s_call)) {               // a library call's result: the number of its name and options
+            Ref number = attr(call, s_number);
+            if (number && number.p == Py_None) number = Ref(PyObject_CallMethodNoArgs(call, s_key));
+            if (!number) return nullptr;
+            k.b.push_back('k');
+            ok = k.integer(number.p) && k.integer(get(s_index));
+        } else {
             Ref s(PyObject_CallMethodNoArgs(op, s_sig));
             if (!s) return nullptr;
             if (s.p == Py_None) Py_RETURN_NONE;
@@ -1496,6 +1511,7 @@ PyMethodDef methods[] = {
     {"plan", py_plan, METH_VARARGS, "plan(slots, needs_ptr, produce, scalars, cleared, Buffer, scalar_value): a plan for replay"},
     {"replay", (PyCFunction)(void (*)(void))py_replay, METH_FASTCALL, "replay(plan, ops, recording): gives results their buffers and issues recorded launches; the library's status"},
     {"set_launch", py_set_launch, METH_O, "takes the address of mjt_record_launch"},
+    {"number_var", (PyCFunction)(void (*)(void))py_number_var, METH_FASTCALL, "number_var(host, dtype): a Var of one number, which goes into kernels by value"},
     {"kernel_var", (PyCFunction)(void (*)(void))py_kernel_var, METH_FASTCALL, "kernel_var(type, call, index, inputs, shape, dtype): a result of a library call"},
     {"gradients", (PyCFunction)(void (*)(void))py_gradients, METH_FASTCALL, "gradients(loss, targets, others): a gradient per target"},
     {"setup", py_setup, METH_O, "takes the classes and tables of core.py"},

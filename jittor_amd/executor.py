@@ -730,13 +730,12 @@ def run_sync(targets, device_sync=False):
         stats["syncs"] += 1
         ops = _pending_ops(targets)
         if ops:
-            target_ids = {t.id for t in targets}
             sig = _graph.signature(ops, targets, flags) if flags["enable_replay"] and _cap is None and _profiler.active() is None else None
             plan = _plans.get(sig) if sig is not None else False
             if plan is None:
-                _capture(ops, target_ids, sig)
+                _capture(ops, {t.id for t in targets}, sig)
             elif plan is False:
-                _execute(ops, target_ids)
+                _execute(ops, {t.id for t in targets})
             else:
                 try:
                     _replay(plan, ops)
@@ -746,9 +745,10 @@ def run_sync(targets, device_sync=False):
                     # a call that is handed back now was not when the plan was made (no workspace left, another MJT_ variable):
                     # the graph is worked out anew
                     _plans.pop(sig, None)
-                    _capture(ops, target_ids, sig)
+                    _capture(ops, {t.id for t in targets}, sig)
         for t in targets:
-            t._device_ptr()
+            if t._buf is None:
+                t._device_ptr()
     if device_sync:
         _lib.sync()
 

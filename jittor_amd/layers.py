@@ -72,10 +72,8 @@ def _number(value, name):
     """64 bits that go into the kernel by value."""
     if not isinstance(value, numbers.Integral):
         raise TypeError("dropout: %s has to be an integer, got %r" % (name, value))
-    v = Var([1], "int64", None, 1)
-    v._host = np.array([int(value) & (1 << 64) - 1], np.uint64).view(np.int64)
-    v.is_scalar = True
-    return v
+    value = int(value) & (1 << 64) - 1
+    return _graph.number_var(np.array([value - (value >> 63 << 64)], np.int64), "int64")
 
 
 def dropout(x, p, is_train, seed, offset, residual):
