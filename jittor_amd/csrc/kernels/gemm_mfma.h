@@ -68,7 +68,8 @@
 //
 // RAGGED 1: rows of any length that begin anywhere (at an element); loads of 16 bytes need no alignment here.  A chunk that a row's end cuts is
 // loaded element by element in the last stage of a sum; of an operand with m or n innermost, which has at least EPC columns, the last
-// EPC columns are loaded instead and go to their own places, where the chunk before writes the same.
+// EPC columns are loaded instead and go to their own places, where the chunk before writes the same.  Loads that cross a line bound it (us a b, as they
+// lie / from padded copies: bfloat16 64 x 10000 x 1001 14.5 / 24.1, 777 x 5200 x 1001 51.6 / 42.4; float32 1024 x 2754 x 513 35.1 / 44.7).
 
 #if IN == 2
 typedef float TIN;

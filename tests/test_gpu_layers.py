@@ -554,7 +554,8 @@ def test_gated_in_blocks_of_rows_without_memory_for_all(gpu):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("ta,tb", [(0, 0), (1, 0), (0, 1)])
-@pytest.mark.parametrize("m,n,k", [(70, 9, 65), (9, 70, 400), (8, 8, 33), (5, 300, 77), (300, 7, 129), (129, 131, 127), (257, 385, 1001), (1, 1, 1), (3, 2, 9), (64, 71, 4099), (700, 1030, 61)])
+@pytest.mark.parametrize("m,n,k", [(70, 9, 65), (9, 70, 400), (8, 8, 33), (5, 300, 77), (300, 7, 129), (129, 131, 127), (257, 385, 1001), (1, 1, 1), (3, 2, 9), (64, 71, 4099), (700, 1030, 61), (1027, 515, 901), (1030, 1099, 259),
+                                    (2563, 1290, 133)])
 def test_products_of_rows_of_any_length(gpu, dtype, ta, tb, m, n, k):
     """Operands whose rows are no whole 16-byte pieces, as they lie where they have k innermost or a piece of columns; an infinity behind the
     last element of each is no part of it."""
@@ -574,6 +575,27 @@ def test_products_of_rows_of_any_length(gpu, dtype, ta, tb, m, n, k):
     got = (bf16_bits_to_f32(got) if dtype == "bfloat16" else got).astype(np.float64)
     _check(got[:m * n].reshape(m, n), a @ b, (k + 2) * E * (np.abs(a) @ np.abs(b)), dtype, (ta, tb))
     assert (got[m * n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ta,tb", [(0, 0), (1, 0), (0, 1)])
+@pytest.mark.parametrize("m,n,k", [(131, 261, 1031), (1027, 515, 901)])
+def test_infinities_stay_in_their_rows_and_columns(gpu, dtype, ta, tb, m, n, k):
+    """Rows of any length with an infinity in the last place of one operand and a NaN in the other's: nothing else is touched."""
+    import ctypes
+    rng = np.random.default_rng(9)
+    a, b = rng.standard_normal((m, k)), rng.standard_normal((k, n))
+    a[m - 1, k - 1], b[0, n - 1] = np.inf, np.nan
+    (ra, ae), (rb, be) = P.to_type(a.T.copy() if ta else a, dtype), P.to_type(b.T.copy() if tb else b, dtype)
+    (x, y, c) = (jt.from_storage(r, dtype) for r in (ra, rb, P.to_type(np.zeros((m, n)), dtype)[0]))
+    pc = c.raw_ptr()
+    gpu.check(gpu.load().mjt_matmul_nearest(*[ctypes.byref(gpu.tensor(p, dtype, s)) for p, s in ((x.raw_ptr(), ra.shape), (y.raw_ptr(), rb.shape), (pc, (m, n)))], ta, tb))
+    assert "_ragged" in gpu.last_kernel()
+    got = gpu.d2h(pc, [m, n], ra.dtype)
+    got = (bf16_bits_to_f32(got) if dtype == "bfloat16" else got).astype(np.float64)
+    ae, be = ae.T if ta else ae, be.T if tb else be
+    _check(got[:-1, :-1], ae[:-1] @ be[:, :-1], (k + 2) * E * (np.abs(ae[:-1]) @ np.abs(be[:, :-1])), dtype, (ta, tb))
+    assert np.array_equal(got[-1, :-1], np.copysign(np.inf, be[-1, :-1])) and np.isnan(got[:, -1]).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
