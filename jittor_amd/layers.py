@@ -140,10 +140,10 @@ def head_norm_rope(who, x, counts, scales, table, positions, sections, eps, inte
         raise ValueError("%s: heads of %d elements (an even number is needed)" % (who, D))
     inputs = [x]
     if scales is not None:
-        scales = [_float_var(who, s, "a scale") for s in scales]
-        if any(s.num != D or s.dtype != scales[0].dtype for s in scales):
-            raise ValueError("%s: scales of %s elements for heads of %d, of one dtype" % (who, [s.num for s in scales], D))
-        inputs += scales
+        q, k = _float_var(who, scales[0], "a scale"), _float_var(who, scales[1], "a scale")
+        if q.num != D or k.num != D or q.dtype != k.dtype:
+            raise ValueError("%s: scales of %s elements for heads of %d, of one dtype" % (who, [q.num, k.num], D))
+        inputs += q, k
     elif table is None:
         raise ValueError("%s: neither scales nor a table: nothing to do" % who)
     if table is not None:
@@ -162,14 +162,15 @@ def head_norm_rope(who, x, counts, scales, table, positions, sections, eps, inte
         if table is None or positions.dtype != "int32":
             raise ValueError("%s: positions are int32 and need a table, got %s" % (who, positions.dtype))
         axes = [] if sections is None else [len(sections)]
-        if list(positions.shape) not in (axes + lead + [S], axes + [S]):
-            raise ValueError("%s: positions %s for tokens %s%s" % (who, list(positions.shape), lead + [S], " with %d axes" % axes[0] if axes else ""))
+        at = list(positions.shape)
+        if at != axes + lead + [S] and at != axes + [S]:
+            raise ValueError("%s: positions %s for tokens %s%s" % (who, at, lead + [S], " with %d axes" % axes[0] if axes else ""))
         inputs.append(positions)
     elif table is not None and S > table.shape[0]:
         raise ValueError("%s: %d tokens and a table of %d positions" % (who, S, table.shape[0]))
     if not float(eps) >= 0.0:
         raise ValueError("%s: eps has to be at least 0, got %r" % (who, eps))
-    call = Call("head_norm_rope", tuple(int(n) for n in counts), scales is not None, table is not None, positions is not None, sections, float(eps), bool(interleaved), bool(heads_first))
+    call = Call("head_norm_rope", tuple(map(int, counts)), scales is not None, table is not None, positions is not None, sections, float(eps), bool(interleaved), bool(heads_first))
     return [_result(call, i, inputs, lead + ([n, S, D] if heads_first else [S, n, D]), x.dtype) for i, n in enumerate(counts) if n]
 
 
