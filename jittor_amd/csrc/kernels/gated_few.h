@@ -1,16 +1,21 @@
 // Gated projections of up to 16 rows: y[m][f] = act(sum_k x[m][k] g[f][k]) * (sum_k x[m][k] u[f][k]), weights [2 F][K] = g above u.
 //
-// The weights are read once and that bounds it: a workgroup owns 8 columns f, eight rows of g and the same rows of u, which are the sixteen
-// rows of one MFMA operand, and its W waves share the sum: pieces of 64 bytes of every row go to the waves in turn, UN of them at a time, so
-// that a workgroup walks along its rows in runs of W * UN * 64 bytes.  A piece is the operand as it lies in memory: lane (row = lane % 16, part = lane / 16)
-// loads 16 bytes, the 8 consecutive k (4 for float32) of its row and part.  The rows of x are the other operand, loaded the
-// same way from the caches.  (float32: a lane's four k feed four MFMAs of 4 k each; both operands use the same pairing.)  The waves' sums meet
-// in LDS, where gate and up of a result meet too.
+// The weights are read once and that bounds it: a workgroup owns 8 columns f, eight rows of g and the same rows of u, and its W waves share the
+// sum: runs of UN * 128 bytes of every row go to the waves in turn.
+// 16 bits: a load of a wave is 128 bytes, a whole line, of each of the eight rows, lane (row = lane % 8, part = lane / 8) the part's 16 bytes.  As an operand of a 16 x 16
+// MFMA those are sixteen rows, each row of weights twice: its even parts and its odd ones.  The operand of x has the even parts of x's rows in one
+// load and the odd ones in another, and is multiplied with both: of the results of the even parts the first eight rows count, of the odd ones the
+// others, and the two halves of a wave add them up.  Half of the products are thrown away; the matrix units have time.  (A piece of 64 bytes of each of the
+// sixteen rows of g and u a load, every product used: lines come in halves, which loads past the caches pay for twice; us so / now, one row of x and weights that are
+// not in the caches: 4096 -> 11264 37.3 / 32.9, 5120 -> 13824 55.1 / 45.8, 2560 -> 6912 20.0 / 15.6.)
+// float32: the products take four times as long, so the rows of g and of u are the sixteen rows of one operand and every product counts; a load is 64
+// bytes of each row, through the caches, where the other half of the line waits for the next (4096 -> 4096 27.3 us, 30.8 past them).  A lane's four k feed four MFMAs of 4 k each; both
+// operands use the same pairing.
+// The waves' sums meet in LDS, where gate and up of a result meet too.
 //
-// us a call over weights that are not in the caches, floor at the rate of a large copy (5.19 TB/s): bfloat16 1 x 4096 -> 11264 37.0, 35.6; 8 x 2048 -> 5632 12.6, 8.9;
-// 1 x 8192 -> 1024 12.5, 6.5.  With sixteen rows of g and of u a workgroup and four waves 37.9 / 14.3 / 24.6: half as many workgroups leave
-// some compute units with twice the others' work.  Four pieces at a time instead of two 38 / 13.2 / 14.0.  More than sixteen rows of x this way
-// wait for x: 24 x 2048 -> 5632 16.5, 64 x 4096 -> 11264 74; those go to tiles.
+// us a call over weights that are not in the caches, floor at the rate of a large copy (5.19 TB/s; reads alone are faster): bfloat16 1 x 4096 -> 11264 32.8, 35.6; 1 x 5120 -> 13824
+// 48.3, 54.6; 8 x 2048 -> 5632 12.0, 8.9; 1 x 8192 -> 1024, 128 workgroups on 256 units, 14.4, 6.5; float32 1 x 2048 -> 8192 24.8, 25.9.  With sixteen rows of g and of u a
+// workgroup half as many workgroups leave some compute units with twice the others' work.  More rows of x wait for x: 16 x 4096 -> 11264 48.4; those go to tiles.
 //
 // Supplied by the host: TYPE, ACT, W, UN, BOTH (gate and up are wanted), Y (y is wanted), RAGGED (otherwise rows of x
 // and of the weights are multiples of 16 bytes and begin at one).  Rows past the last are read from the last, their results are not stored.
@@ -26,8 +31,9 @@ typedef float mjt_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 mjt_b16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 mjt_h16x8 __attribute__((ext_vector_type(8)));
 #define EPL (TYPE == 2 ? 4 : 8)          // elements of a lane's 16 bytes
-#define STEP (4 * EPL)                   // k of a piece
+#define STEP (8 * EPL)                   // k of a line of 128 bytes
 
+template <int V> struct mjt_ic { static constexpr int v = V; };
 __device__ __forceinline__ mjt_f32x4 mjt_multiply(mjt_piece a, mjt_piece b, mjt_f32x4 c) {
 #if TYPE == 0
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mjt_b16x8, a), __builtin_bit_cast(mjt_b16x8, b), c, 0, 0, 0);
@@ -44,39 +50,81 @@ extern "C" __global__ __launch_bounds__(W * 64) void ENTRY(Params p) {
     typedef typename mjt_el<TYPE>::raw raw;
     const int M = (int)(long long)p.a[4], F = (int)(long long)p.a[5], K = (int)(long long)p.a[6];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = lane & 15, at = (lane >> 4) * EPL;
-    const long long f0 = (long long)blockIdx.x * 8, f = f0 + row % 8 < F ? f0 + row % 8 : F - 1;
-    const raw* w = (const raw*)p.a[1] + ((row < 8 ? 0 : (long long)F) + f) * K + at;
-    const raw* x = (const raw*)p.a[0] + (long long)(row < M ? row : M - 1) * K + at;
-    mjt_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    int k = wave * (UN * STEP);
-    for (; k + UN * STEP <= K; k += W * UN * STEP) {
-        mjt_piece a[UN], b[UN];
-#pragma unroll
-        for (int u = 0; u < UN; u++) {
-            a[u] = __builtin_nontemporal_load((const mjt_there*)(w + k + u * STEP));
-            b[u] = *(const mjt_there*)(x + k + u * STEP);
-        }
-#pragma unroll
-        for (int u = 0; u < UN; u++) acc = mjt_multiply(a[u], b[u], acc);
-    }
-    // the last run of the row ends with one of the waves: piece by piece, nothing past K
-    for (int end = k + UN * STEP; k < end && k < K; k += STEP) {
-        const int have = K - k - at;                           // elements that the lane's piece has
-        mjt_piece a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-        if (have >= EPL) a = *(const mjt_there*)(w + k), b = *(const mjt_there*)(x + k);
+    const int m16 = lane & 15, half = lane >> 4;
+    const long long f0 = (long long)blockIdx.x * 8;
+    const raw* x = (const raw*)p.a[0] + (long long)(m16 < M ? m16 : M - 1) * K;
+    __shared__ float part[W][16][20];
+    // fullc: the piece lies inside the row; otherwise what is behind its end is zero
+    auto piece = [&](const raw* row, int k, auto fullc) {
+        mjt_piece v = {0, 0, 0, 0};
+        if (decltype(fullc)::v || k + EPL <= K) v = *(const mjt_there*)(row + k);
 #if RAGGED
         else
 #pragma unroll
             for (int j = 0; j < EPL; j++)
-                if (j < have) ((raw*)&a)[j] = w[k + j], ((raw*)&b)[j] = x[k + j];
+                if (k + j < K) ((raw*)&v)[j] = row[k + j];
 #endif
-        acc = mjt_multiply(a, b, acc);
-    }
-    // D of a 16 x 16 tile: lane holds column lane % 16 (a row of x), rows 4 * (lane / 16) + e (g, then u)
-    __shared__ float part[W][16][20];
+        return v;
+    };
+#if TYPE == 2
+    const long long f = f0 + lane % 8 < F ? f0 + lane % 8 : F - 1;
+    const raw* w = (const raw*)p.a[1] + (m16 < 8 ? f : F + f) * K;
+    mjt_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto run = [&](int k, auto nc, auto fullc) {
+        constexpr int N = decltype(nc)::v;
+        mjt_piece a[2 * N], b[2 * N];
 #pragma unroll
-    for (int e = 0; e < 4; e++) part[wave][4 * (lane >> 4) + e][row] = acc[e];
+        for (int i = 0; i < 2 * N; i++) {
+            a[i] = piece(w, k + i * STEP / 2 + half * EPL, fullc);
+            b[i] = piece(x, k + i * STEP / 2 + half * EPL, fullc);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * N; i++) acc = mjt_multiply(a[i], b[i], acc);
+    };
+#else
+    const long long f = f0 + lane % 8 < F ? f0 + lane % 8 : F - 1;
+    const raw *g = (const raw*)p.a[1] + f * K, *u = g + (long long)F * K;
+    mjt_f32x4 ge = {0.0f, 0.0f, 0.0f, 0.0f}, go = ge, ue = ge, uo = ge;           // even and odd parts
+    auto run = [&](int k, auto nc, auto fullc) {
+        constexpr int N = decltype(nc)::v;
+        mjt_piece a[N], b[N], even[N], odd[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int kw = k + i * STEP + (lane >> 3) * EPL, kx = k + i * STEP + half * (2 * EPL);
+            if (decltype(fullc)::v) {
+                a[i] = __builtin_nontemporal_load((const mjt_there*)(g + kw));
+                b[i] = __builtin_nontemporal_load((const mjt_there*)(u + kw));
+            } else {
+                a[i] = piece(g, kw, fullc);
+                b[i] = piece(u, kw, fullc);
+            }
+            even[i] = piece(x, kx, fullc);
+            odd[i] = piece(x, kx + EPL, fullc);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            ge = mjt_multiply(a[i], even[i], ge);
+            go = mjt_multiply(a[i], odd[i], go);
+            ue = mjt_multiply(b[i], even[i], ue);
+            uo = mjt_multiply(b[i], odd[i], uo);
+        }
+    };
+#endif
+    int k = wave * (UN * STEP);
+    for (; k + UN * STEP <= K; k += W * UN * STEP) run(k, mjt_ic<UN>(), mjt_ic<1>());
+    for (int end = k + UN * STEP; k < end && k < K; k += STEP) run(k, mjt_ic<1>(), mjt_ic<0>());      // (the last run of a row: it ends with one of the waves)
+    // D of a 16 x 16 tile: lane holds column lane % 16 (a row of x), rows 4 * (lane / 16) + e
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+#if TYPE == 2
+        part[wave][4 * half + e][m16] = acc[e];
+#else
+        float gate = half < 2 ? ge[e] : go[e], up = half < 2 ? ue[e] : uo[e];
+        gate += __shfl_xor(gate, 32, 64);
+        up += __shfl_xor(up, 32, 64);
+        part[wave][(half < 2 ? 0 : 8) + 4 * (half & 1) + e][m16] = half < 2 ? gate : up;
+#endif
+    }
     __syncthreads();
     const int c = threadIdx.x % 8, m = threadIdx.x / 8;
     if (m >= M || f0 + c >= F) return;

@@ -37,11 +37,12 @@ void rows_pass(int act, const void* both, const void* y, const void* d, int dtyp
 }
 
 // The ways to run the projections, by estimated time.
-//   FEW (kernels/gated_few.h): up to 16 rows.  16-bit operands of more than 4 rows and 24 MB of weights are better off on tiles, which load x once
-//   for 32 columns (us few / MFMA: 16 x 1024 -> 2816 6.4 / 7.4; 16 x 2048 -> 5632 14.7 / 10.8, of 4 rows 11.9 / 11.1); float32 MFMAs are slower
-//   than the loads of x (float32 16 x 2048 -> 5632 28 / 33).  Rows that are no whole 16-byte pieces: up to 20 MB, as their loads cross lines (us few / MFMA or PRODUCT:
-//   bfloat16 1 x 1501 -> 1500 6.3 / 9.8, of 16 rows 9.2 / 12.8, 1 x 2231 -> 2610 14.6 / 13.3, of 16 26.1 / 17.8; float32 4 x 1501 -> 1500 8.4 / 12.8, 4 x 2231 -> 2610 22.3 / 19.5).
-//   TILES (kernels/gemm_dma.h): 16-bit operands on 256 x 256 tiles, one to a compute unit, or 128 x 128, two to a unit.
+//   FEW (kernels/gated_few.h): up to 8 rows, and up to 16 where x is not the longer way: float32, whose MFMAs of other routes wait as well, and up to 48 MB of 16-bit weights
+//   (us few / MFMA or TILES, weights not in the caches: bfloat16 8 x 4096 -> 11264 39.3 / 41.4, 8 x 2048 -> 5632 12.0 / 15.2, 16 x 2048 -> 5632 14.1 / 15.4, on the other side 16 x 4096 ->
+//   11264 48.4 / 42.3, 16 x 2560 -> 6912 22.8 / 18.5; float32 16 x 4096 -> 4096 38.7 / 42.5).  Rows that are no whole 16-byte pieces, whose loads cross lines: 16 bits up to 20 MB,
+//   float32 up to 8 rows or 48 MB (bfloat16 4 x 1501 -> 1500 9.7 / 12.3, 4 x 2231 -> 2610 22.3 / 16.7; float32 4 x 4001 -> 9001 84.8 / 98.3, 16 x 4001 -> 9001 114.7 / 99.8).
+//   TILES (kernels/gemm_dma.h): 16-bit operands on 256 x 256 tiles, one to a compute unit, or 128 x 128, two to a unit.  Up to 128 rows only the latter (128 x 8192 -> 28672 235 /
+//   188), up to 64 none: MFMA has tiles of 64 rows (us TILES / MFMA: 64 x 5120 -> 13824 62.9 / 57.5, 64 x 1536 -> 8960 20.1 / 18.9, 24 x 4096 -> 11264 42.2 / 42.1).
 //   MFMA (kernels/gemm_mfma.h): any type and rows of any length; a product that is better cut into slices of its sum goes to PRODUCT, the plain product in
 //   32 bits and a pass over it (before rows of any length ran here, us then / now: bfloat16 36 x 46 -> 256 23 / 5.7, 777 x 1001 -> 2600 42.1 / 32.8, 4000 x 45 -> 3001 67.7 / 30.7;
 //   float32 3722 x 99 -> 3968 135 / 101, 1024 x 513 -> 1377 45.5 / 30.2).
@@ -61,22 +62,29 @@ Route choose(int dtype, int64_t M, int64_t F, int64_t K, bool aligned, int* tile
     const double stages = std::ceil((double)K / 64.0);
     auto rounds = [&](double tiles, double at_once) { return std::ceil(tiles / at_once); };
     auto tiles_of = [&](int64_t rows, int64_t cols) { return (double)((M + rows - 1) / rows) * (double)((F + cols - 1) / cols); };
-    if (may("few") && M <= 16 && F < (int64_t(1) << 25) && (forced || (aligned ? esz == 4 || M <= 4 || bytes <= int64_t(24) << 20 : bytes <= int64_t(20) << 20))) return FEW;
+    const int64_t mb = int64_t(1) << 20;
+    const bool few = aligned ? M <= 8 || esz == 4 || bytes <= 48 * mb : esz == 2 ? bytes <= 20 * mb : M <= 8 || bytes <= 48 * mb;
+    if (may("few") && M <= 16 && F < (int64_t(1) << 25) && (forced || few)) return FEW;
     if (may("tiles") && aligned && esz == 2 && K >= 64 && K * 2 * 256 < (int64_t(1) << 31)) {
         const double r256 = rounds(tiles_of(256, 128), (double)cus), n128 = tiles_of(128, 64), r128 = rounds(n128, 2.0 * (double)cus);
         const double t256 = r256 * (10.0 + 1.1 * stages) * (r256 > 1 ? 1.2 : 1.0);
         const double t128 = n128 <= (double)cus ? 5.3 + 0.335 * stages : r128 * (6.0 + 0.66 * stages * (1.0 + std::max(0.0, stages - 32.0) / 64.0)) * (r128 > 1 && stages >= 32.0 ? 1.2 : 1.0);
         const double mfma = 3.5 + 0.25 * stages * (1.0 + 0.8 * (rounds(tiles_of(64, 32), (double)cus) - 1.0));
-        *tile = t256 < t128 ? 256 : 128;
+        *tile = M > 128 && t256 < t128 ? 256 : 128;
         if (const char* e = getenv("MJT_GEMM_DMA")) *tile = atoi(e) == 128 ? 128 : 256;
-        if (forced || std::min(t256, t128) < mfma) return TILES;
+        if (forced || (M > 64 && (*tile == 256 ? t256 : t128) < mfma)) return TILES;
     }
     return may("mfma") ? MFMA : PRODUCT;
 }
 
 void few_rows(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
     const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2;
-    const int W = 8, UN = 2;
+    // Lines of 128 bytes that a wave takes at a time: the most for which every wave has the same number of runs (us for 1 / 2 / 4, bfloat16, one row, weights not in
+    // the caches: 4096 -> 11264 34.4 / 34.1 / 32.2, 4096 -> 14336 45.6 / 44.8 / 38.3, 5120 -> 13824 48.0 / 44.1 / 46.2, 2560 -> 6912 14.5 / 14.7 / 15.9, 1536 -> 8960 11.6 / 11.8 / 13.0).
+    // Four waves instead of eight: 37.9 / 36.0 / 37.3 for the first of these, 8192 -> 1024 20.3 instead of 12.6.
+    const int W = 8;
+    const int64_t turn = W * 128 / dtype_size(x->dtype);
+    const int UN = K % (4 * turn) == 0 ? 4 : K % (2 * turn) == 0 ? 2 : 1;
     const bool ragged = K * dtype_size(x->dtype) % 16 != 0 || (uintptr_t)x->ptr % 16 != 0 || (uintptr_t)w->ptr % 16 != 0;
     std::ostringstream name, defs;
     name << "mjt_gated_few_" << act_name(act) << "_" << mjt_dtype_name(x->dtype) << (ragged ? "_ragged" : "") << (both ? y ? "_both" : "_products" : "");

@@ -324,17 +324,18 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
 bool gemm_gated(int dtype, int act, const char* act_name, const void* x, const void* w, void* y, void* both, int64_t M, int64_t F, int64_t K) {
     const int esz = dtype_size(dtype);
     TileChoice t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 2 * F);
+    const bool ragged = K * esz % 16 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0;
     // A sum in slices needs the plain product, a launch that adds them up and one for the activation; of 16-bit operands it is worth that from 48
     // stages on (us in slices / whole: bfloat16 24 x 2048 -> 261 12.6 / 10.3, 252 x 2584 -> 896 15.2 / 12.4, 600 x 3000 -> 300 17.2 / 14.1, on the other side 1247 x 3952
-    // -> 56 12.1 / 15.7, 130 x 4096 -> 130 10.3 / 16.7; float32 103 x 1584 -> 50 11.0 / 29.6).
-    if (t.slices > 1 && esz == 2 && t.stages < 48) t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 0);
+    // -> 56 12.1 / 15.7, 130 x 4096 -> 130 10.3 / 16.7; float32 103 x 1584 -> 50 11.0 / 29.6; rows of any
+    // length 4 x 2231 -> 2610 16.7 / 23.3).
+    if (t.slices > 1 && esz == 2 && !ragged && t.stages < 48) t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 0);
     if (t.slices > 1) return false;
     t.mi = std::min(t.mi, 2);                                   // (a tile's results have to fit its LDS)
     t.ni = std::min(t.ni, 2);
     const int in = dtype == MJT_BFLOAT16 ? 0 : dtype == MJT_FLOAT16 ? 1 : 2, gated = (y ? 1 : 0) + (both ? 2 : 0);
     const bool one_stage = t.stages == 1 && t.mi * t.ni == 1;
     const int vs = F % 4 == 0 && (uintptr_t)y % (size_t)(4 * esz) == 0 && (uintptr_t)both % 16 == 0 ? 4 : 1;
-    const bool ragged = K * esz % 16 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0;
     std::ostringstream name, defs;
     name << "mjt_gated_mfma_" << act_name << "_" << mjt_dtype_name(dtype) << "_" << 64 * t.mi << "x" << 64 * t.ni << (one_stage ? "_k1" : "") << (t.split ? "_parts" : "") << (ragged ? "_ragged" : "") << (both ? y ? "_both" : "_products" : "");
     defs << "#define RAGGED " << (ragged ? 1 : 0) << "\n#define NBUF " << (one_stage ? 1 : 2) << "\n#define SPLIT " << (t.split ? 1 : 0) << "\n#define IN " << in << "\n#define OUT 2\n#define MI " << t.mi << "\n#define NI " << t.ni
