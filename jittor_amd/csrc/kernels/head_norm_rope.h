@@ -30,10 +30,16 @@ typedef typename mjt_el<TYPE>::raw raw;
 typedef typename mjt_el<STYPE>::raw raws;
 #define R (64 / LP)                    // rows of a wave
 
-// whether every axis ends with a whole chunk of V pairs
+// A chunk's V pairs are one group of neighbours; or with PAIRED, where both elements of a pair lie in one piece, one of each piece, which are then half a
+// row apart if they are whole 16-byte accesses: side by side every access of a wave takes half of each line, and those past the caches read
+// lines twice (us side by side / apart: 48 heads of 128 bfloat16, 8192 tokens 47.4 / 38.9, 48 heads of 64 float32, 4096 tokens 23.4 / 19.8, gradient 32.5 / 26.9).
+// Smaller pieces side by side are one access (24 heads of 80 bfloat16 on three axes, 9477 tokens 18.0 / 18.7, gradient 30.5 / 32.1).
+constexpr int GN = PAIRED && V * sizeof(raw) >= 16 ? 2 : 1, G = V / GN;
+
+// whether every axis ends with a whole group
 template <int N> constexpr bool mjt_whole(const int (&ends)[N]) {
     for (int a = 0; a < N; a++)
-        if (ends[a] % V) return false;
+        if (ends[a] % G) return false;
     return true;
 }
 template <int CTRL> __device__ __forceinline__ float mjt_dpp(float v) { return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CTRL, 0xf, 0xf, true)); }
@@ -64,17 +70,22 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
     const float eps = (float)__longlong_as_double((long long)p.a[13]);
     const raw* __restrict__ x = (const raw*)p.a[0];
     // the lane's pieces of a row: V elements from first[c] and from second[c] on; chunks past the row are those of chunk 0 and count nothing
-    int first[NC], second[NC], pair[NC];
-    bool in[NC], turned[NC];
+    int first[NC], second[NC], pair[NC][GN];
+    bool in[NC], turned[NC][GN];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         int at = (c * LP + own) * V;
         in[c] = at < D / 2;
         at = in[c] ? at : 0;
-        turned[c] = ROT > 0 && at < ROT / 2;
-        pair[c] = turned[c] ? at : 0;
-        first[c] = turned[c] && !PAIRED ? at : 2 * at;
-        second[c] = turned[c] && !PAIRED ? at + ROT / 2 : 2 * at + V;
+        const bool halves = GN == 2 || (!PAIRED && ROT > 0 && at < ROT / 2);          // one piece in front, the other behind
+        first[c] = halves ? at : 2 * at;
+        second[c] = halves ? at + (GN == 2 ? D : ROT) / 2 : 2 * at + V;
+#pragma unroll
+        for (int g = 0; g < GN; g++) {
+            const int p0 = GN == 2 ? (g ? second[c] : first[c]) / 2 : at;
+            turned[c][g] = p0 < ROT / 2;
+            pair[c][g] = turned[c][g] ? p0 : 0;
+        }
     }
     // element i of piece e of a chunk, e and i of pair j's two elements: its piece's j-th each, or (neighbours) elements 2 j and 2 j + 1 of the 2 V
     constexpr auto piece = [](int j, int e) { return PAIRED ? (2 * j + e) / V : e; };
@@ -107,30 +118,32 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
 #endif
             constexpr bool whole = mjt_whole(ends);
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                if constexpr (whole) {                          // the chunk's pairs lie on one axis
-                    unsigned row = at[0];
+            for (int c = 0; c < NC; c++)
 #pragma unroll
-                    for (int a = 1; a < AXES; a++) row = pair[c] >= ends[a - 1] ? at[a] : row;
-                    const bool there = row < rows;
-                    const mjt_els<2, 2 * V> f = *(const mjt_els<2, 2 * V>*)(table + ((long long)(there ? row : 0) * (ROT / 2) + pair[c]) * 2);
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        cs[c][i] = turned[c] ? there ? f.v[2 * i] : __builtin_nanf("") : 1.0f;
-                        sn[c][i] = turned[c] ? f.v[2 * i + 1] : 0.0f;
-                    }
-                } else
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
+                for (int g = 0; g < GN; g++) {
+                    if constexpr (whole) {                      // the group's pairs lie on one axis
                         unsigned row = at[0];
 #pragma unroll
-                        for (int a = 1; a < AXES; a++) row = pair[c] + i >= ends[a - 1] ? at[a] : row;
+                        for (int a = 1; a < AXES; a++) row = pair[c][g] >= ends[a - 1] ? at[a] : row;
                         const bool there = row < rows;
-                        const float* f = table + ((long long)(there ? row : 0) * (ROT / 2) + pair[c] + i) * 2;
-                        cs[c][i] = turned[c] ? there ? f[0] : __builtin_nanf("") : 1.0f;
-                        sn[c][i] = turned[c] ? f[1] : 0.0f;
-                    }
-            }
+                        const mjt_els<2, 2 * G> f = *(const mjt_els<2, 2 * G>*)(table + ((long long)(there ? row : 0) * (ROT / 2) + pair[c][g]) * 2);
+#pragma unroll
+                        for (int i = 0; i < G; i++) {
+                            cs[c][g * G + i] = turned[c][g] ? there ? f.v[2 * i] : __builtin_nanf("") : 1.0f;
+                            sn[c][g * G + i] = turned[c][g] ? f.v[2 * i + 1] : 0.0f;
+                        }
+                    } else
+#pragma unroll
+                        for (int i = 0; i < G; i++) {
+                            unsigned row = at[0];
+#pragma unroll
+                            for (int a = 1; a < AXES; a++) row = pair[c][g] + i >= ends[a - 1] ? at[a] : row;
+                            const bool there = row < rows;
+                            const float* f = table + ((long long)(there ? row : 0) * (ROT / 2) + pair[c][g] + i) * 2;
+                            cs[c][g * G + i] = turned[c][g] ? there ? f[0] : __builtin_nanf("") : 1.0f;
+                            sn[c][g * G + i] = turned[c][g] ? f[1] : 0.0f;
+                        }
+                }
         }
 #else
 #pragma unroll
