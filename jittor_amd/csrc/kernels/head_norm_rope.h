@@ -34,7 +34,8 @@ typedef typename mjt_el<STYPE>::raw raws;
 // row apart if they are whole 16-byte accesses: side by side every access of a wave takes half of each line, and those past the caches read
 // lines twice (us side by side / apart: 48 heads of 128 bfloat16, 8192 tokens 47.4 / 38.9, 48 heads of 64 float32, 4096 tokens 23.4 / 19.8, gradient 32.5 / 26.9).
 // Smaller pieces side by side are one access (24 heads of 80 bfloat16 on three axes, 9477 tokens 18.0 / 18.7, gradient 30.5 / 32.1).
-constexpr int GN = PAIRED && V * sizeof(raw) >= 16 ? 2 : 1, G = V / GN;
+constexpr bool APART = V * sizeof(raw) >= 16;
+constexpr int GN = PAIRED && APART ? 2 : 1, G = V / GN;
 
 // whether every axis ends with a whole group
 template <int N> constexpr bool mjt_whole(const int (&ends)[N]) {
@@ -77,9 +78,10 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
         int at = (c * LP + own) * V;
         in[c] = at < D / 2;
         at = in[c] ? at : 0;
-        const bool halves = GN == 2 || (!PAIRED && ROT > 0 && at < ROT / 2);          // one piece in front, the other behind
-        first[c] = halves ? at : 2 * at;
-        second[c] = halves ? at + (GN == 2 ? D : ROT) / 2 : 2 * at + V;
+        // pieces of a pair's halves; of neighbours, or of what is not turned, in front and behind where they are whole accesses, otherwise side by side
+        const bool halves = !PAIRED && at < ROT / 2;
+        first[c] = halves || GN == 2 ? at : APART ? at + ROT / 2 : 2 * at;
+        second[c] = halves ? at + ROT / 2 : APART ? at + D / 2 : 2 * at + V;
 #pragma unroll
         for (int g = 0; g < GN; g++) {
             const int p0 = GN == 2 ? (g ? second[c] : first[c]) / 2 : at;

@@ -116,8 +116,12 @@ Plan plan_for(const char* who, const mjt_tensor* x, const mjt_tensor* q_scale, c
     a.V = V;
     a.LP = LP;
     a.NC = (int)NC;
-    // (past the caches only whole lines: 8192 tokens of 48 heads of 128 bfloat16 41.8 / 38.4 us, but 9477 of 24 heads of 80 17.4 / 22.9)
-    const bool far = D * esz % 128 == 0 && streams(a.tokens * H * D * esz * (back ? 3 : 2));
+    // Past the caches where every access of a wave takes whole lines of the rows, whose pieces lie as the kernel says (us through / past them: 8192 tokens of 48
+    // heads of 128 bfloat16 42.2 / 38.3, gradient 63.6 / 59.6, on the other side 96 heads of 64 44.7 / 47.7 and 66.0 / 70.1, 48 of 128 with 64 elements turned 42.4 / 43.2, 9477
+    // of 24 heads of 80 17.4 / 22.9); the gradient of heads turned in part also otherwise (48 of 128 with 64 turned 77.7 / 67.4).
+    auto lines = [&](int64_t elements) { return elements * esz % 128 == 0; };
+    const bool apart = V * esz >= 16, whole = p->interleaved ? lines(apart ? D / 2 : D) : lines(rot / 2) && lines(apart ? (D - rot) / 2 : D - rot);
+    const bool far = (whole || (back && rot < D && lines(D))) && streams(a.tokens * H * D * esz * (back ? 3 : 2));
     std::ostringstream defs;
     defs << "#define STREAMS " << (far ? 1 : 0) << "\n#define TYPE " << a.type << "\n#define STYPE " << a.scale_type << "\n#define D " << D << "\n#define ROT " << rot << "\n#define V " << V << "\n#define LP " << LP << "\n#define NC " << NC
          << "\n#define PAIRED " << (p->interleaved ? 1 : 0) << "\n#define FIRST " << (p->heads_first ? 1 : 0) << "\n#define NORM " << (q_scale ? 1 : 0) << "\n#define AXES " << axes

@@ -229,6 +229,14 @@ def test_passes_larger_than_the_caches_keep(gpu, dtype):
     _heads(dtype, (1, 1003), 40, 3, 192, 48, False, True, seed=16)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("paired", [False, True])
+@pytest.mark.parametrize("dim,pairs", [(128, 64), (128, 32), (256, 64), (128, 0), (64, 32)])
+def test_layouts_of_large_passes(gpu, dtype, paired, dim, pairs):
+    """Pieces of rows side by side and half a row apart, turned whole, in part and not at all."""
+    _heads(dtype, (2, 190000 // dim), 16, 4, dim, pairs, paired, True, seed=dim + pairs)
+
+
 def test_without_rotation_without_norm_and_with_scales_of_another_type(gpu):
     _heads("bfloat16", (2, 6), 4, 2, 64, 0, False, False)
     _heads("bfloat16", (2, 6), 4, 2, 64, 32, False, True, scaled=False)
