@@ -51,7 +51,7 @@ extern "C" __global__ __launch_bounds__(W * 64) void ENTRY(Params p) {
     const int M = (int)(long long)p.a[4], F = (int)(long long)p.a[5], K = (int)(long long)p.a[6];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m16 = lane & 15, half = lane >> 4;
-    const long long f0 = (long long)blockIdx.x * 8;
+    const long long f0 = (long long)blockIdx.x * 8, f = f0 + lane % 8 < F ? f0 + lane % 8 : F - 1;
     const raw* x = (const raw*)p.a[0] + (long long)(m16 < M ? m16 : M - 1) * K;
     __shared__ float part[W][16][20];
     // fullc: the piece lies inside the row; otherwise what is behind its end is zero
@@ -67,7 +67,6 @@ extern "C" __global__ __launch_bounds__(W * 64) void ENTRY(Params p) {
         return v;
     };
 #if TYPE == 2
-    const long long f = f0 + lane % 8 < F ? f0 + lane % 8 : F - 1;
     const raw* w = (const raw*)p.a[1] + (m16 < 8 ? f : F + f) * K;
     mjt_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     auto run = [&](int k, auto nc, auto fullc) {
@@ -82,7 +81,6 @@ extern "C" __global__ __launch_bounds__(W * 64) void ENTRY(Params p) {
         for (int i = 0; i < 2 * N; i++) acc = mjt_multiply(a[i], b[i], acc);
     };
 #else
-    const long long f = f0 + lane % 8 < F ? f0 + lane % 8 : F - 1;
     const raw *g = (const raw*)p.a[1] + f * K, *u = g + (long long)F * K;
     mjt_f32x4 ge = {0.0f, 0.0f, 0.0f, 0.0f}, go = ge, ue = ge, uo = ge;           // even and odd parts
     auto run = [&](int k, auto nc, auto fullc) {
