@@ -81,7 +81,7 @@ struct TileChoice {
     int64_t slices, per, stages;
     bool split;
 };
-static TileChoice choose_tiles(int in_dtype, int64_t M, int64_t N, int64_t K, int64_t batch, bool a_kcont, bool b_kcont, int tile_m, int tile_n, int64_t ldc) {
+static TileChoice choose_tiles(int in_dtype, int64_t M, int64_t N, int64_t K, int64_t batch, bool a_kcont, bool b_kcont, int tile_m, int tile_n, int64_t ldc, bool layers) {
     Context& c = ctx();
     const int esz = dtype_size(in_dtype);
     // Tile: the largest of 64 MI x 64 NI (MI, NI in 1, 2, 4) that still gives every compute unit work and wastes
@@ -117,6 +117,9 @@ static TileChoice choose_tiles(int in_dtype, int64_t M, int64_t N, int64_t K, in
     auto crowd = [&](double wgs) { const double r = std::ceil(wgs / cus); return 1.0 + 0.8 * (r - 1.0); };
     const double st = esz == 2 ? 0.5 : 0.75;
     double least = (double)stages * st * crowd(tiles64) * (best_mi * best_ni > 1 ? 0.95 : 1.0);
+    // Several rounds of float32 tiles take a fifth longer than that; products of the layers' operators go by it (us float32 MFMAs / parts: a^T b 20096 x 704 x 322
+    // 107 / 90, 16640 x 512 x 478 92 / 82, gated 700 x 256 -> 5000 41.3 / 34.0), others keep the sums they had.
+    if (layers && in_dtype == MJT_FLOAT32 && tiles64 > (double)cus) least *= 1.2;
     // float32 sums of four stages and more go as products of bfloat16 parts (kernels/gemm_mfma.h) on 128 x 64, 64 x 128 or
     // 128 x 128 tiles, whole or in slices, where that is estimated to take less.  A stage takes 0.92 us on 128 x 64 tiles and 1.45
     // on 128 x 128, a little more where an operand is transposed on the way; a round of workgroups adds a first load and a
@@ -252,7 +255,7 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
         }
     }
     if (fast || ragged) {
-        const TileChoice chosen = choose_tiles(in_dtype, M, N, K, batch, a_kcont, b_kcont, tile_m, tile_n, ldc);
+        const TileChoice chosen = choose_tiles(in_dtype, M, N, K, batch, a_kcont, b_kcont, tile_m, tile_n, ldc, Nearest::on());
         const int best_mi = chosen.mi, best_ni = chosen.ni;
         int64_t slices = chosen.slices;
         const int64_t per = chosen.per, stages = chosen.stages;
@@ -323,13 +326,13 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
 
 bool gemm_gated(int dtype, int act, const char* act_name, const void* x, const void* w, void* y, void* both, int64_t M, int64_t F, int64_t K) {
     const int esz = dtype_size(dtype);
-    TileChoice t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 2 * F);
+    TileChoice t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 2 * F, true);
     const bool ragged = K * esz % 16 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0;
     // A sum in slices needs the plain product, a launch that adds them up and one for the activation; of 16-bit operands it is worth that from 48
     // stages on (us in slices / whole: bfloat16 24 x 2048 -> 261 12.6 / 10.3, 252 x 2584 -> 896 15.2 / 12.4, 600 x 3000 -> 300 17.2 / 14.1, on the other side 1247 x 3952
     // -> 56 12.1 / 15.7, 130 x 4096 -> 130 10.3 / 16.7; float32 103 x 1584 -> 50 11.0 / 29.6; rows of any
     // length 4 x 2231 -> 2610 16.7 / 23.3).
-    if (t.slices > 1 && esz == 2 && !ragged && t.stages < 48) t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 0);
+    if (t.slices > 1 && esz == 2 && !ragged && t.stages < 48) t = choose_tiles(dtype, M, 2 * F, K, 1, true, true, 0, 0, 0, true);
     if (t.slices > 1) return false;
     t.mi = std::min(t.mi, 2);                                   // (a tile's results have to fit its LDS)
     t.ni = std::min(t.ni, 2);
