@@ -585,6 +585,27 @@ def test_products_of_rows_of_any_length(gpu, dtype, ta, tb, m, n, k):
     assert (got[m * n:] == 7.0).all()
 
 
+@pytest.mark.parametrize("ta,tb", [(0, 0), (1, 0), (0, 1)])
+@pytest.mark.parametrize("m,n,k", [(2563, 1290, 61), (2560, 1280, 64), (2048, 1412, 96), (1290, 2563, 33), (2100, 1300, 127)])
+def test_short_sums_on_large_tiles(gpu, ta, tb, m, n, k):
+    """Two to four stages of float32 as bfloat16 parts, and one value that needs the float32 loop."""
+    import ctypes
+    rng = np.random.default_rng(k)
+    a, b = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((k, n)).astype(np.float32)
+    a[7, k - 1] = np.inf
+    x, y = jt.array(a.T.copy() if ta else a), jt.array(b.T.copy() if tb else b)
+    c = core.Var([m, n], "float32")
+    c._buf = core.Buffer(c.nbytes)
+    gpu.check(gpu.load().mjt_matmul_nearest(*[ctypes.byref(gpu.tensor(v.raw_ptr(), "float32", v.shape)) for v in (x, y)], ctypes.byref(gpu.tensor(c._buf.ptr, "float32", c.shape)), ta, tb))
+    assert "128x128" in gpu.last_kernel() and "_parts" in gpu.last_kernel()
+    got = gpu.d2h(c._buf.ptr, [m, n], np.float32).astype(np.float64)
+    assert np.array_equal(got[7], np.copysign(np.inf, b[-1].astype(np.float64)))
+    a[7, k - 1] = 0.0
+    rows = np.arange(m) != 7
+    a64, b64 = a[rows].astype(np.float64), b.astype(np.float64)
+    _check(got[rows], a64 @ b64, (k + 2) * E * (np.abs(a64) @ np.abs(b64)), "float32", (ta, tb))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("ta,tb", [(0, 0), (1, 0), (0, 1)])
 @pytest.mark.parametrize("m,n,k", [(131, 261, 1031), (1027, 515, 901)])
