@@ -1059,7 +1059,9 @@ def _execute(ops, target_ids):
             if op.id in absorbed_nodes:
                 continue
             if isinstance(op, KernelOp):
-                same = next((c for c in calls if c[0].call is op.call and all(a is b for a, b in zip(c[0].inputs, op.inputs))), None)
+                # (a result that was made twice, by two threads that take gradients of one call, takes two launches)
+                same = next((c for c in calls if c[0].call is op.call and all(a is b for a, b in zip(c[0].inputs, op.inputs))
+                             and all(o.index != op.index for o in c)), None)
                 if same is not None:
                     same.append(op)
                     same_task[id(same)].writes.add(op.out.id)

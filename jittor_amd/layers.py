@@ -7,6 +7,7 @@ when they are asked for.
 import ctypes
 import itertools
 import numbers
+import weakref
 
 import numpy as np
 
@@ -23,10 +24,11 @@ _numbers, _next = {}, itertools.count()            # (name, options) -> its numb
 
 class Call:
     """What is called and with which options; shared by the ops of its results."""
-    __slots__ = ("name", "options", "number")
+    __slots__ = ("name", "options", "number", "kept")
 
     def __init__(self, name, *options):
         self.name, self.options, self.number = name, options, None
+        self.kept = None                                       # weakly, a result that gradients read and nobody else has
 
     def key(self):
         """A number for name and options: a graph's key is worked out and looked up for every execution."""
@@ -250,8 +252,12 @@ def _gated_gradients(op, inputs, douts, wanted):
     x, w = inputs
     dy = douts[0]
     f2 = w.shape[0]
-    # the products of the forward pass in 32 bits: written by the same launch where the two passes run together, made again otherwise
-    both = _result(op.call, 1, list(inputs), list(x.shape[:-1]) + [f2], "float32")
+    # the products of the forward pass in 32 bits: written by the same launch where the two passes run together, made again otherwise.  Gradients that
+    # are taken one after the other share them for as long as any that reads them waits.
+    both = op.call.kept() if op.call.kept is not None else None
+    if both is None:
+        both = _result(op.call, 1, list(inputs), list(x.shape[:-1]) + [f2], "float32")
+        op.call.kept = weakref.ref(both)
     d = _result(Call("gated_linear_grad", *op.call.options), 0, [dy, both], list(x.shape[:-1]) + [f2], dy.dtype)
     return [_result(Call("product", False, False), 0, [d, w], list(x.shape), x.dtype) if wanted[0] else None,
             _result(Call("product", True, False), 0, [d, x], list(w.shape), w.dtype) if wanted[1] else None]

@@ -496,6 +496,28 @@ def test_gradients_asked_for_after_the_result_has_been_computed(gpu):
     _check(_got(dw), dwe, dwo, "float16", "dw")
 
 
+@pytest.mark.parametrize("replay", [True, False])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_gradients_of_one_gated_layer_taken_one_by_one(gpu, replay, dtype):
+    """Two calls of grad() over one layer, then one sync or two: the values of a single call, and of two losses each its own."""
+    rng = np.random.default_rng(41)
+    with jt.flag_scope(enable_replay=replay):
+        for turn in range(4):
+            (x, xe), (w, we) = _make(rng, (21, 40), dtype), _make(rng, (2 * 24, 40), dtype, 0.2)
+            (g, ge), (h, he) = _make(rng, (21, 24), dtype), _make(rng, (21, 24), dtype)
+            y = jt.nn.gated_linear(x, w)
+            loss, other = (y * g).sum(), (y * h).sum()
+            dx, dw = jt.grad(loss, x), jt.grad(loss, w)
+            hx, hw = jt.grad(other, [x, w])
+            if turn % 2:
+                jt.sync([dw])
+            jt.sync([hw, dx, dw, hx])
+            for e, (ux, uw) in ((ge, (dx, dw)), (he, (hx, hw))):
+                (want_x, off_x), (want_w, off_w) = P.gated_grad(xe, we, "silu", e, dtype)
+                _check(_got(ux), want_x, off_x, dtype, ("dx", turn))
+                _check(_got(uw), want_w, off_w, dtype, ("dw", turn))
+
+
 def test_gated_replays(gpu):
     rng = np.random.default_rng(7)
     w, we = _make(rng, (256, 128), "bfloat16", 0.1)

@@ -1,13 +1,14 @@
 """Operators of transformer layers without a GPU: the plain forms that the GPU tests compare with, refusals, kernels that build for every
 type, the ops that gradients are made of."""
 import ctypes
+import gc
 
 import numpy as np
 import pytest
 
 import jittor_amd as jt
 from jittor_amd import _lib as L
-from jittor_amd import core, layers
+from jittor_amd import core, executor, layers
 import layers_plain as P
 
 B = ctypes.byref
@@ -268,3 +269,62 @@ def test_a_feed_forward_layer_keeps_its_type(dtype):
     x, w, o = _x(3, 4, dtype=dtype), _x(6, 4, dtype=dtype), _x(5, 3, dtype=dtype)
     y = jt.nn.gated_ffn(x, w, o)
     assert y.dtype == dtype and y.shape == [3, 5] and [g.dtype for g in jt.grad(y.sum(), [x, w, o])] == [dtype] * 3
+
+
+# ---- graphs of gradients, executed up to the launches -------------------------------------------------------------------
+@pytest.fixture
+def launches(compile_only, monkeypatch):
+    """Graphs are executed in compile-only mode on addresses that nothing is read from; what is launched is listed."""
+    class Pool:
+        at = 1 << 20
+
+        def alloc(self, n):
+            Pool.at += 1 << 20
+            return Pool.at, n
+
+        def free(self, ptr, size):
+            pass
+
+    listed, launch = [], layers.launch
+    monkeypatch.setenv("MJT_NO_DISK_CACHE", "1")
+    monkeypatch.setattr(core, "pool", Pool())
+    monkeypatch.setattr(layers, "launch", lambda ex, ops: (listed.append((ops[0].call.name, sorted(op.index for op in ops))), launch(ex, ops)))
+    yield listed
+    executor._plans.clear()
+    gc.collect()                                            # (buffers go back to the pool they are from)
+
+
+def _there(*shape):
+    v = core.Var(list(shape), "float32")
+    v._buf = core.Buffer(4 * v.num)
+    return v
+
+
+def test_gradients_of_one_gated_result_taken_one_by_one(launches):
+    """Two calls of grad() and one sync: both read the same products of the forward pass, which are made once."""
+    x, w = _there(3, 4), _there(6, 4)
+    y = jt.nn.gated_linear(x, w)
+    loss = (y * _there(3, 3)).sum()
+    gx, gw = jt.grad(loss, x), jt.grad(loss, w)
+    jt.sync([gx, gw])
+    assert gx._op is None and gw._op is None
+    assert sorted(launches) == [("gated_linear", [1])] + 2 * [("gated_linear_grad", [0])] + 2 * [("product", [0])]
+
+
+def test_two_losses_over_a_shared_gated_layer(launches):
+    x, w = _there(3, 4), _there(6, 4)
+    y = jt.nn.gated_linear(x, w)
+    grads = [g for k in range(2) for g in jt.grad((y * _there(3, 3)).sum(), [x, w])]
+    jt.sync([y] + grads)
+    assert all(v._op is None for v in [y] + grads)
+    assert sorted(launches) == [("gated_linear", [0, 1])] + 2 * [("gated_linear_grad", [0])] + 4 * [("product", [0])]
+
+
+def test_a_result_that_was_asked_for_twice_is_made_twice(launches):
+    """Whoever makes the same result of one call a second time gets it, whatever else is pending."""
+    x, w = _there(3, 4), _there(6, 4)
+    y = jt.nn.gated_linear(x, w)
+    again = [layers._result(y._op.call, 1, [x, w], [3, 6], "float32") for _ in range(2)]
+    jt.sync([y] + again)
+    assert y._op is None and all(v._op is None and v._buf is not None for v in again)
+    assert sorted(launches) == [("gated_linear", [0, 1]), ("gated_linear", [1])]
