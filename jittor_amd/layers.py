@@ -4,6 +4,7 @@ Each is a call of the library (include/mjt.h) with one or several results, a cor
 programs use are in nn.py.  Their gradients are calls of the same kind.  Second derivatives are not there: they are refused
 when they are asked for.
 """
+import copy
 import ctypes
 import itertools
 import numbers
@@ -60,6 +61,8 @@ class _Generator:
         self.seed(0)
 
     def seed(self, seed):
+        if not isinstance(seed, numbers.Integral):             # what else numpy makes a generator of: a copy's first number, the generator itself goes on from where it is
+            seed = copy.deepcopy(np.random.default_rng(seed)).integers(1 << 63)
         self.state = int(seed), itertools.count()              # (one object: threads that draw at the same time get numbers of one key)
 
     def next(self):

@@ -97,6 +97,22 @@ def test_a_seed_numbers_the_calls_without_one():
     jt.set_seed(0)
 
 
+@pytest.mark.parametrize("seed", [lambda: None, lambda: [1, 2], lambda: np.random.SeedSequence(4), lambda: np.random.default_rng(3), lambda: np.random.PCG64(3), lambda: np.uint64(1 << 63)],
+                         ids=["none", "list", "sequence", "generator", "bits", "uint64"])
+def test_seeds_are_what_numpy_takes(seed):
+    """jt.random's numbers are numpy's for the seed; dropout numbers its calls anew, the same again where the seed says what the numbers are."""
+    def draws(s):
+        jt.set_seed(s)
+        return jt.random([5]).numpy(), [tuple(int(u._host[0]) for u in jt.nn.dropout(_x(4), 0.5, True)._op.inputs[1:]) for _ in range(2)]
+    (r, (first, second)), (again, calls) = draws(seed()), draws(seed())
+    jt.set_seed(0)
+    assert first[1:] == (0,) and second == (first[0], 1)
+    if seed() is None:
+        assert not np.array_equal(r, again) and calls[0] != first
+    else:
+        assert np.array_equal(r, np.random.default_rng(seed()).random(5).astype(np.float32)) and np.array_equal(r, again) and calls == [first, second]
+
+
 @pytest.mark.parametrize("case", [
     dict(qkv=(4, 8)), dict(qkv=(2, 4, 7, 8)), dict(qkv=(2, 4, 6, 7)), dict(heads=0), dict(kv=0), dict(k_scale=False), dict(q_scale=False), dict(scale=(9,)), dict(scale_dtype="float16"),
     dict(table=(10, 5, 2)), dict(table=(10, 4, 3)), dict(table=(0, 4, 2)), dict(table_dtype="float16"), dict(positions=(2, 3)), dict(positions_dtype="float32"),
