@@ -443,6 +443,9 @@ int mjt_fused_reindex_reduce_then(const mjt_fused_desc* desc, const mjt_tensor* 
  * (MJT_VAR_SCALAR vars whose ivalue holds 64 bits), so that the gradient is
  * the same call on dy with residual NULL. */
 int mjt_dropout(const mjt_tensor* x, const mjt_tensor* residual, const mjt_tensor* y, double p, const mjt_fused_var* key, const mjt_fused_var* call);
+/* The same by numbers of their own, which no key and call give mjt_dropout:
+ * for calls that a program does not number itself. */
+int mjt_dropout_unnumbered(const mjt_tensor* x, const mjt_tensor* residual, const mjt_tensor* y, double p, const mjt_fused_var* key, const mjt_fused_var* call);
 
 /* x [.., tokens, heads, dim] with the heads of queries, keys and values side
  * by side: q and k are normalised by the root of their mean square for each

@@ -104,7 +104,7 @@ EXPORTS = ["mjt_init", "mjt_shutdown", "mjt_last_error", "mjt_get_device_info",
            "mjt_fused_elementwise", "mjt_fused_reduce", "mjt_fused_rows", "mjt_conv2d_meta", "mjt_conv2d_meta_pack", "mjt_conv2d_meta_packed", "mjt_conv2d_meta_grouped", "mjt_conv2d_meta_dgrad", "mjt_conv2d_meta_dgrad_depthwise", "mjt_conv2d_meta_wgrad", "mjt_conv2d_meta_wgrad_grouped",
            "mjt_reindex_then_reduce", "mjt_fused_reindex_reduce", "mjt_matmul", "mjt_matmul_available",
            "mjt_conv2d_meta_backward_depthwise", "mjt_conv2d_meta_then", "mjt_conv2d_meta_dgrad_then", "mjt_matmul_then", "mjt_fused_reindex_reduce_then",
-           "mjt_dropout", "mjt_head_norm_rope", "mjt_head_norm_rope_grad", "mjt_gated_linear", "mjt_gated_linear_grad", "mjt_matmul_nearest",
+           "mjt_dropout", "mjt_dropout_unnumbered", "mjt_head_norm_rope", "mjt_head_norm_rope_grad", "mjt_gated_linear", "mjt_gated_linear_grad", "mjt_matmul_nearest",
            "mjt_expr_affine", "mjt_where_count", "mjt_where",
            "mjt_record_begin", "mjt_record_end", "mjt_record_relocate", "mjt_record_launch", "mjt_record_free",
            "mjt_jit_stats", "mjt_last_kernel"]
@@ -177,6 +177,7 @@ def load():
     lib.mjt_matmul_then.argtypes = lib.mjt_matmul.argtypes + [ctypes.POINTER(FusedDesc)]
     t = ctypes.POINTER(Tensor)
     lib.mjt_dropout.argtypes = [t, t, t, ctypes.c_double, ctypes.POINTER(FusedVar), ctypes.POINTER(FusedVar)]
+    lib.mjt_dropout_unnumbered.argtypes = lib.mjt_dropout.argtypes
     lib.mjt_head_norm_rope.argtypes = [t] * 5 + [ctypes.POINTER(HeadNorm)] + [t] * 3
     lib.mjt_head_norm_rope_grad.argtypes = [t] * 5 + [ctypes.POINTER(HeadNorm)] + [t] * 6
     lib.mjt_gated_linear.argtypes = [t, t, ctypes.c_int, t, t]

@@ -2,15 +2,15 @@
 //
 // keep(e) is u(e) >= T with T = round(p * 2^32) and a number u(e) of 32 bits that depends on the element's place, the key and the call
 // alone, so the mask is never stored: the backward pass works it out again.  u comes from Philox4x32 with 10 rounds (J. Salmon,
-// M. Moraes, R. Dror and D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011), whose counter is (e / 8, block, call): a
+// M. Moraes, R. Dror and D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011), whose counter is (e / 8, side and block, call): a
 // block of 128 bits gives the upper 16 bits of eight neighbouring elements' numbers (word e / 2 % 4, the lower half for even e), a second block their
 // lower 16.  The upper halves decide unless one of them equals T / 2^16, one element in 65536, so that a wave works out the second block
 // for one pass in 128 (never where T's lower half is 0, p = 0.5 or 0.25): full resolution of p for half the arithmetic.
 // A dropped element is 0 whatever it held, also an infinity or NaN.
 //
 // Supplied by the host: TYPE (element type), RES, WIDE (a lane's eight elements are whole aligned vectors), STREAMS.
-// a[0] x  a[1] residual  a[2] y  a[3] elements  a[4] key  a[5] call  a[6] T  a[7] 1 / (1 - p) (double bits)
-struct Params { void* a[8]; };
+// a[0] x  a[1] residual  a[2] y  a[3] elements  a[4] key  a[5] call  a[6] T  a[7] 1 / (1 - p) (double bits)  a[8] the side, in place in the counter's second word
+struct Params { void* a[9]; };
 
 struct mjt_u4 { unsigned w[4]; };
 // ten rounds of two multiplications of 32 bits to 64 and the key's Weyl steps
@@ -30,10 +30,10 @@ __device__ __forceinline__ mjt_u4 mjt_philox(unsigned c0, unsigned c1, unsigned 
 __device__ __forceinline__ unsigned mjt_half_of(const mjt_u4& w, int j) { return j & 1 ? w.w[j / 2] >> 16 : w.w[j / 2] & 0xffffu; }
 
 // bit j: element j of group g is kept
-__device__ __forceinline__ unsigned mjt_keep_bits(unsigned long long g, unsigned long long key, unsigned long long call, unsigned long long threshold) {
+__device__ __forceinline__ unsigned mjt_keep_bits(unsigned long long g, unsigned long long key, unsigned long long call, unsigned long long threshold, unsigned side) {
     const unsigned hi = (unsigned)(threshold >> 16), lo = (unsigned)(threshold & 0xffffu);        // hi up to 65536, for p = 1
     const unsigned k0 = (unsigned)key, k1 = (unsigned)(key >> 32), c2 = (unsigned)call, c3 = (unsigned)(call >> 32);
-    const mjt_u4 a = mjt_philox((unsigned)g, (unsigned)(g >> 32), c2, c3, k0, k1);
+    const mjt_u4 a = mjt_philox((unsigned)g, (unsigned)(g >> 32) | side, c2, c3, k0, k1);
     unsigned keep = 0, tie = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -42,7 +42,7 @@ __device__ __forceinline__ unsigned mjt_keep_bits(unsigned long long g, unsigned
         tie |= (u == hi ? 1u : 0u) << j;
     }
     if (lo != 0 && __any(tie != 0)) {
-        const mjt_u4 b = mjt_philox((unsigned)g, (unsigned)(g >> 32) | 0x80000000u, c2, c3, k0, k1);
+        const mjt_u4 b = mjt_philox((unsigned)g, (unsigned)(g >> 32) | side | 0x80000000u, c2, c3, k0, k1);
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if ((tie >> j & 1) && mjt_half_of(b, j) < lo) keep &= ~(1u << j);
@@ -71,7 +71,7 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
                 if (RES) add.v[j] = j < have ? res[g * 8 + j] : raw(0);
             }
         }
-        const unsigned keep = threshold ? mjt_keep_bits((unsigned long long)g, key, call, threshold) : 0xffu;
+        const unsigned keep = threshold ? mjt_keep_bits((unsigned long long)g, key, call, threshold, (unsigned)(unsigned long long)p.a[8]) : 0xffu;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             float v = keep >> j & 1 ? mjt_el<TYPE>::up(in.v[j]) * scale : 0.0f;

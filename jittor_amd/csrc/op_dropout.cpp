@@ -6,7 +6,8 @@
 
 namespace mjt {
 
-static void dropout_impl(const mjt_tensor* x, const mjt_tensor* residual, const mjt_tensor* y, double p, const mjt_fused_var* key, const mjt_fused_var* call) {
+// side: bits 28 to 30 of the counter's second word, which no element's place reaches
+static void dropout_impl(const mjt_tensor* x, const mjt_tensor* residual, const mjt_tensor* y, double p, const mjt_fused_var* key, const mjt_fused_var* call, uint64_t side) {
     require_init();
     check_tensor(x, "dropout: x");
     check_tensor(y, "dropout: y");
@@ -29,11 +30,14 @@ static void dropout_impl(const mjt_tensor* x, const mjt_tensor* residual, const 
     const int64_t groups = (n + 7) / 8, blocks = std::min((groups + 255) / 256, int64_t(1) << 23);
     const uint64_t threshold = (uint64_t)std::nearbyint(p * 4294967296.0);
     jit_launch(k, (unsigned)blocks, 1, 256, 0, {bits_of_ptr(x->ptr), bits_of_ptr(residual ? residual->ptr : nullptr), bits_of_ptr(y->ptr), (uint64_t)n, (uint64_t)key->ivalue,
-                                              (uint64_t)call->ivalue, threshold, bits_of(p < 1.0 ? 1.0 / (1.0 - p) : 0.0)});
+                                              (uint64_t)call->ivalue, threshold, bits_of(p < 1.0 ? 1.0 / (1.0 - p) : 0.0), side << 28});
 }
 
 }  // namespace mjt
 
 extern "C" int mjt_dropout(const mjt_tensor* x, const mjt_tensor* residual, const mjt_tensor* y, double p, const mjt_fused_var* key, const mjt_fused_var* call) {
-    return mjt::guarded([&] { mjt::dropout_impl(x, residual, y, p, key, call); });
+    return mjt::guarded([&] { mjt::dropout_impl(x, residual, y, p, key, call, 0); });
+}
+extern "C" int mjt_dropout_unnumbered(const mjt_tensor* x, const mjt_tensor* residual, const mjt_tensor* y, double p, const mjt_fused_var* key, const mjt_fused_var* call) {
+    return mjt::guarded([&] { mjt::dropout_impl(x, residual, y, p, key, call, 1); });
 }

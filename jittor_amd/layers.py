@@ -96,30 +96,32 @@ def dropout(x, p, is_train, seed, offset, residual):
         if residual is None:
             return x
         p, seed, offset = 0.0, 0, 0                            # (the sum alone, rounded as in training)
-    elif seed is None:
+    numbered = seed is not None                                # by the program; otherwise by numbers that no seed and offset of a program's give
+    if not numbered:
         seed, offset = generator.next()
     key = [_number(seed, "the seed"), _number(offset or 0, "the offset")]
     inputs = [x] + ([] if residual is None else [residual]) + key
-    return _result(Call("dropout", p, residual is not None), 0, inputs, list(x.shape), x.dtype)
+    return _result(Call("dropout", p, residual is not None, numbered), 0, inputs, list(x.shape), x.dtype)
 
 
 def _launch_dropout(ex, options, inputs, outs):
-    p, added = options
+    p, added, numbered = options
     x, y = inputs[0], outs[0]
     scalars = [(_lib.FusedVar * 1)(_lib.FusedVar(_lib.VAR_SCALAR, _lib.DTYPE_CODE["int64"], None, 0.0, int(u._host.reshape(-1)[0]))) for u in inputs[-2:]]
     if ex._cap is not None:
         ex._cap.scalars += [(s, 0, u) for s, u in zip(scalars, inputs[-2:])]
     tx, ty = ex._tensor_of(x), ex._tensor(ex._alloc_out(y), y.dtype, y.shape)
     res = ctypes.byref(ex._tensor_of(inputs[1])) if added else None
-    _lib.check(ex._libh().mjt_dropout(ctypes.byref(tx), res, ctypes.byref(ty), p, *scalars))
+    lib = ex._libh()
+    _lib.check((lib.mjt_dropout if numbered else lib.mjt_dropout_unnumbered)(ctypes.byref(tx), res, ctypes.byref(ty), p, *scalars))
 
 
 def _dropout_gradients(op, inputs, douts, wanted):
-    p, added = op.call.options
+    p, added, numbered = op.call.options
     dy = douts[0]
     grads = [None] * len(inputs)
     if wanted[0]:
-        grads[0] = _result(Call("dropout", p, False), 0, [dy] + list(inputs[-2:]), list(dy.shape), dy.dtype) if p else dy
+        grads[0] = _result(Call("dropout", p, False, numbered), 0, [dy] + list(inputs[-2:]), list(dy.shape), dy.dtype) if p else dy
     if added and wanted[1]:
         grads[1] = dy
     return grads

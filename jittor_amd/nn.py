@@ -228,7 +228,7 @@ def dropout(x, p=0.5, is_train=False, seed=None, offset=None, residual=None):
 
     The mask is never stored: it depends on the elements' places, `seed` and `offset` (integers of 64 bits) alone, and the gradient works
     it out again.  Calls of one program that are to be independent differ in one of the two; without a seed the generator of jt.set_seed
-    numbers the calls.  A dropped element is 0 whatever it held."""
+    numbers the calls, whose numbers no seed and offset give.  A dropped element is 0 whatever it held."""
     return layers.dropout(x, p, is_train, seed, offset, residual)
 
 

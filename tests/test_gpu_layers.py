@@ -80,6 +80,25 @@ def test_dropout_at_the_threshold(gpu):
         assert np.array_equal(_got(y) != 0, u >= t), t
 
 
+@pytest.mark.parametrize("p", [0.5, 0.3])
+def test_calls_without_a_seed_have_numbers_of_their_own(gpu, p):
+    """Neither the i-th call behind set_seed(s) nor its gradient has the mask of seed s and offset i: bit 28 of the counter's second word tells them apart."""
+    n = 8 * 50
+    x = jt.array(np.ones(n, np.float32))
+    jt.set_seed(9)
+    for call in range(3):
+        y = jt.nn.dropout(x, p, True)
+        dx = jt.grad(y.sum(), x)
+        u = []
+        for g in range(n // 8):
+            hi, lo = (P.philox([g, 1 << 28 | block << 31, call, 0], [9, 0]) for block in (0, 1))
+            u += [((hi[j // 2] >> 16 * (j % 2)) & 0xFFFF) << 16 | (lo[j // 2] >> 16 * (j % 2)) & 0xFFFF for j in range(8)]
+        keep = np.array(u, np.uint64) >= round(p * 2.0 ** 32)
+        assert np.array_equal(_got(y) != 0, keep) and np.array_equal(_got(dx) != 0, keep)
+        assert not np.array_equal(keep, P.kept(n, p, 9, call))
+    jt.set_seed(0)
+
+
 def test_dropped_infinities_and_nan_are_zero(gpu):
     n, p = 4096, 0.3
     keep = P.kept(n, p, 1, 0)

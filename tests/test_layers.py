@@ -97,6 +97,17 @@ def test_a_seed_numbers_the_calls_without_one():
     jt.set_seed(0)
 
 
+def test_numbers_of_calls_without_a_seed_are_not_those_of_one(launches):
+    """The key and number of a call without a seed may be a program's own seed and offset: its numbers, and its gradient's, are others."""
+    jt.set_seed(0)
+    x, taken = _there(4, 4), []
+    for y in (jt.nn.dropout(x, 0.5, True), jt.nn.dropout(x, 0.5, True, seed=0)):
+        dx = jt.grad((y * _there(4, 4)).sum(), x)
+        taken.append({(op.call.name, op.call.options, tuple(int(u._host[0]) for u in op.inputs[1:])) for op in _calls([y, dx])})
+        jt.sync([y, dx])
+    assert all(len(t) == 1 and next(iter(t))[2] == (0, 0) for t in taken) and taken[0] != taken[1]
+
+
 @pytest.mark.parametrize("seed", [lambda: None, lambda: [1, 2], lambda: np.random.SeedSequence(4), lambda: np.random.default_rng(3), lambda: np.random.PCG64(3), lambda: np.uint64(1 << 63)],
                          ids=["none", "list", "sequence", "generator", "bits", "uint64"])
 def test_seeds_are_what_numpy_takes(seed):
