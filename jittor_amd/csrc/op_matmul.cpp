@@ -177,36 +177,25 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
                         M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31);
     std::vector<uint64_t> args{bits_of_ptr(A), bits_of_ptr(B), bits_of_ptr(C), (uint64_t)M, (uint64_t)N, (uint64_t)K,
                                (uint64_t)lda, (uint64_t)ldb, (uint64_t)ldc, (uint64_t)sa, (uint64_t)sb, (uint64_t)sc};
-    // 256 x 256 tiles that fill some rounds of the compute units and less than 0.7 of another: the whole rounds' tile rows first, and
-    // the rest as a product of its own, on the tiles that suit it (us as one / so: bfloat16 a^T b 11264 x 2048 x 8192, 352 tiles, 350 / 314).  For the products
-    // of layers.py's gradients; others keep the sums they had.
-    if (fast && allow_direct && esz == 2 && Nearest::on() && batch == 1 && K % 64 == 0 && K >= 1024 && !tile_m && !tile_n) {
-        const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
-        const int64_t tn = (N + 255) / 256, tiles = (M + 255) / 256 * tn, rows = tiles / cus * cus / tn * 256;
-        if (tiles > cus && tiles % cus && (double)(tiles % cus) < 0.7 * (double)cus && rows > 0 && rows < M && (double)(rows / 256 * tn) >= 0.95 * (double)(tiles / cus * cus)) {
-            const char* rest = (const char*)A + rows * (a_kcont ? lda : 1) * esz;
-            gemm_launch(in_dtype, out_dtype, A, B, C, rows, N, K, lda, ldb, ldc, sa, sb, sc, 1, a_kcont, b_kcont);
-            gemm_launch(in_dtype, out_dtype, rest, B, (char*)C + rows * ldc * dtype_size(out_dtype), M - rows, N, K, lda, ldb, ldc, sa, sb, sc, 1, a_kcont, b_kcont);
-            return;
-        }
-    }
+    const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
     // 16-bit operands, K a multiple of 64 and enough tiles of 256 x 256 to go round: the kernel whose operands reach LDS
     // without passing through registers (any of the four layouts).  Offsets inside an operand's tile are 32-bit there:
     // 256 rows of an operand with k innermost, all K rows of one with m or n innermost.
     auto fits32 = [&](bool kcont, int64_t ld) { return (kcont ? ld * 2 * 256 : ld * 2 * K) < (int64_t(1) << 31); };
-    if (fast && allow_direct && esz == 2 && K % 64 == 0 && !getenv("MJT_GEMM_NO_DMA") && fits32(a_kcont, lda) && fits32(b_kcont, ldb)) {
-        const int64_t cus = c.dry_run || c.prop.multiProcessorCount <= 0 ? 256 : c.prop.multiProcessorCount;
-        // 256 x 256 tiles on two stage buffers, or 128 x 128 tiles on a ring of four (a 128-tile's stage is a quarter of
-        // the MFMA time, so more stages have to be on their way): the smaller tile where the larger one leaves compute
-        // units without work
+    const bool direct = fast && allow_direct && esz == 2 && K % 64 == 0 && !getenv("MJT_GEMM_NO_DMA") && fits32(a_kcont, lda) && fits32(b_kcont, ldb);
+    // The tile of that kernel for `rows` rows of C, 0 for none.
+    // 256 x 256 tiles on two stage buffers, or 128 x 128 tiles on a ring of four (a 128-tile's stage is a quarter of
+    // the MFMA time, so more stages have to be on their way): the smaller tile where the larger one leaves compute
+    // units without work
+    auto direct_tile = [&](int64_t rows) {
         int tile = 0;
         // a caller that names its tile has measured the general kernel against the 256 x 256 tiles; 128 x 128 tiles of this
         // kernel are still better than the general kernel's from two stages on (measured on 1x1 convolutions below)
         const bool hinted = tile_m || tile_n;
         const int smallest = hinted && !(tile_m == 128 && tile_n == 128 && K >= 128) ? 256 : 128;
         for (int t = 256; t >= smallest && !tile; t /= 2) {
-            const int64_t tm = (M + t - 1) / t, tn = (N + t - 1) / t;
-            const double edge = ((double)M * N) / ((double)tm * t * tn * t);
+            const int64_t tm = (rows + t - 1) / t, tn = (N + t - 1) / t;
+            const double edge = ((double)rows * N) / ((double)tm * t * tn * t);
             const double tiles = (double)tm * tn * batch;
             const double util = tiles / (std::ceil(tiles / cus) * cus);
             // (a sum of fewer than four stages does not fill the time a 256 x 256 tile's operands take to arrive, and only
@@ -214,6 +203,23 @@ void gemm_launch(int in_dtype, int out_dtype, const void* A, const void* B, void
             if (edge >= 0.85 && util >= (t == 256 ? 0.7 : 0.25) && (t == 128 || K >= 256)) tile = t;
         }
         if (const char* e = getenv("MJT_GEMM_DMA")) tile = atoi(e) == 128 ? 128 : 256;
+        return tile;
+    };
+    // 256 x 256 tiles that fill some rounds of the compute units and less than 0.7 of another: the whole rounds' tile rows first, where they run on
+    // such tiles, and the rest as a product of its own, on the tiles that suit it (us as one / so: bfloat16 a^T b 11264 x 2048 x 8192, 352 tiles, 350 / 314).  For the
+    // products of layers.py's gradients; others keep the sums they had.
+    if (direct && Nearest::on() && batch == 1 && K >= 1024 && !tile_m && !tile_n) {
+        const int64_t tn = (N + 255) / 256, tiles = (M + 255) / 256 * tn, rows = tiles / cus * cus / tn * 256;
+        if (tiles > cus && tiles % cus && (double)(tiles % cus) < 0.7 * (double)cus && rows > 0 && rows < M && (double)(rows / 256 * tn) >= 0.95 * (double)(tiles / cus * cus) &&
+            direct_tile(rows) == 256) {
+            const char* rest = (const char*)A + rows * (a_kcont ? lda : 1) * esz;
+            gemm_launch(in_dtype, out_dtype, A, B, C, rows, N, K, lda, ldb, ldc, sa, sb, sc, 1, a_kcont, b_kcont);
+            gemm_launch(in_dtype, out_dtype, rest, B, (char*)C + rows * ldc * dtype_size(out_dtype), M - rows, N, K, lda, ldb, ldc, sa, sb, sc, 1, a_kcont, b_kcont);
+            return;
+        }
+    }
+    if (direct) {
+        const int tile = direct_tile(M);
         if (tile) {
             const int64_t tm = (M + tile - 1) / tile, tn = (N + tile - 1) / tile;
             const int in = in_dtype == MJT_BFLOAT16 ? 0 : 1;

@@ -254,6 +254,23 @@ def test_entry_points_refuse(compile_only):
     refused(lib.mjt_gated_linear_grad(B(y), B(y), 0, B(w)))
 
 
+def test_products_are_cut_into_whole_rounds_only_where_those_run_on_large_tiles(compile_only, monkeypatch):
+    """40960 x 336 counts 320 tiles of 256 x 256, more than a round of them, but a third of each row of tiles would be empty: the product runs whole on the
+    tiles that it has where nothing is cut.  What is left of a cut product runs on a kernel of its own (here the ring of four stages of one tile each)."""
+    monkeypatch.setenv("MJT_NO_DISK_CACHE", "1")
+    lib = compile_only.load()
+
+    def kernel(f, m, n, k):
+        L.check(f(B(_t("bfloat16", m, k)), B(_t("bfloat16", k, n)), B(_t("bfloat16", m, n)), 0, 0))
+        return L.last_kernel().replace("_nearest", "")
+
+    whole, rest = kernel(lib.mjt_matmul, 40960, 336, 1024), kernel(lib.mjt_matmul, 8192, 336, 1024)
+    assert whole != rest and kernel(lib.mjt_matmul_nearest, 40960, 336, 1024) == whole
+    monkeypatch.setenv("MJT_GEMM_NO_DMA", "1")               # nor without the kernel of those tiles
+    for n in (336, 512):
+        assert kernel(lib.mjt_matmul_nearest, 40960, n, 1024) == kernel(lib.mjt_matmul, 40960, n, 1024)
+
+
 # ---- graphs of gradients (built, not run) -----------------------------------------------------------------------------------
 def _calls(vs):
     return [op for op in core._graph.pending_ops(vs) if isinstance(op, core.KernelOp)]
