@@ -1,8 +1,8 @@
 """Operators of transformer layers as graph ops: what stands around attention and the plain linear layers.
 
 Each is a call of the library (include/mjt.h) with one or several results, a core.KernelOp for each of them; the functions that
-programs use are in nn.py.  Their gradients are calls of the same kind.  Second derivatives are not there: they are refused
-when they are asked for.
+programs use are in nn.py.  Their gradients are calls of the same kind.  Second derivatives of norms of heads and of gated projections are not
+there: they are refused when they are asked for.
 """
 import copy
 import ctypes
@@ -268,10 +268,25 @@ def _gated_gradients(op, inputs, douts, wanted):
             _result(Call("product", True, False), 0, [d, x], list(w.shape), w.dtype) if wanted[1] else None]
 
 
+def down_projection(x, weight):
+    """x * weight^T for bfloat16, rounded to nearest even like what the other operators here write, gradients too; the ordinary product truncates."""
+    if weight.ndim != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("gated_ffn: the second weight %s has to be [n, %d]" % (list(weight.shape), x.shape[-1]))
+    return _result(Call("product", False, True), 0, [x, weight], list(x.shape[:-1]) + [weight.shape[0]], x.dtype)
+
+
+def _product_gradients(op, inputs, douts, wanted):
+    (a, b), dc = inputs, douts[0]
+    trans_a, trans_b = op.call.options
+    da = ((b, dc) if trans_a else (dc, b)), (False, trans_a or not trans_b)                  # a^T b: b dc^T;  a b^T: dc b;  a b: dc b^T
+    db = ((dc, a) if trans_b else (a, dc)), (not trans_a, False)                             #        a dc;           dc^T a;        a^T dc
+    return [_result(Call("product", *trans), 0, list(ops), list(u.shape), u.dtype) if want else None for u, (ops, trans), want in zip(inputs, (da, db), wanted)]
+
+
 # ---- what the executor and grad() call ------------------------------------------------------------------------------------
 _LAUNCH = {"dropout": _launch_dropout, "head_norm_rope": _launch_head_norm, "head_norm_rope_grad": _launch_head_norm_grad, "gated_linear": _launch_gated,
            "gated_linear_grad": _launch_gated_grad, "product": _launch_product}
-_GRADIENTS = {"dropout": _dropout_gradients, "head_norm_rope": _head_norm_gradients, "gated_linear": _gated_gradients}
+_GRADIENTS = {"dropout": _dropout_gradients, "head_norm_rope": _head_norm_gradients, "gated_linear": _gated_gradients, "product": _product_gradients}
 
 
 def launch(ex, ops):

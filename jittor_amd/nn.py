@@ -270,9 +270,13 @@ def gated_linear(x, weight, activation="silu"):
 
 
 def gated_ffn(x, w_in, w_out, activation="silu"):
-    """The whole feed-forward layer: gated_linear(x, w_in) * w_out^T, w_in [2 f, k], w_out [n, f], in x's type."""
+    """The whole feed-forward layer: gated_linear(x, w_in) * w_out^T, w_in [2 f, k], w_out [n, f], in x's type; each of the two products is rounded to
+    nearest where x is in 16 bits, and so are the gradients."""
+    h, w_out = gated_linear(x, w_in, activation), core._as_var(w_out)
+    if h.dtype == w_out.dtype == "bfloat16":
+        return layers.down_projection(h, w_out)
     with flag_scope(amp_reg=flags.amp_reg | 36):               # (a sum of 16-bit products keeps their type, as a convolution's does)
-        return matmul_transpose(gated_linear(x, w_in, activation), w_out)
+        return matmul_transpose(h, w_out)
 
 
 core.Var.matmul = core.Var.__matmul__ = matmul

@@ -552,6 +552,47 @@ def test_gated_replays(gpu):
         _check(_got(dw), dwe, dwo, "bfloat16", turn)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,f,n", [(1, 64, 48, 40), (37, 33, 21, 19), (200, 128, 96, 136)])
+def test_feed_forward_layers(gpu, dtype, rows, k, f, n):
+    """Both products and all gradients.  Beyond P.gated and P.gated_grad: what arrives at the second product has been rounded to the type, and so has
+    the gradient that arrives at the first."""
+    rng = np.random.default_rng(rows)
+    (x, xe), (w, we), (o, oe), (g, ge) = (_make(rng, s, dtype, c) for s, c in (((rows, k), 1.0), ((2 * f, k), 0.2), ((n, f), 0.3), ((rows, n), 1.0)))
+    y = jt.nn.gated_ffn(x, w, o)
+    assert y.dtype == dtype
+    dx, dw, do = jt.grad((y * g).sum(), [x, w, o])
+    jt.sync([y, dx, dw, do])
+    he, off = P.gated(xe, we, "silu")
+    off = off * (1 + ULP[dtype]) + ULP[dtype] * np.abs(he) + TINY[dtype]
+    size = np.abs(he) + off
+    _check(_got(y), he @ oe.T, off @ np.abs(oe).T + 2 * f * E * (size @ np.abs(oe).T), dtype, "y")
+    _check(_got(do), ge.T @ he, np.abs(ge).T @ off + 2 * rows * E * (np.abs(ge).T @ size), dtype, "dw_out")
+    dh = ge @ oe
+    edh = 2 * n * E * (np.abs(ge) @ np.abs(oe))
+    edh = edh * (1 + ULP[dtype]) + ULP[dtype] * np.abs(dh) + TINY[dtype]
+    (dxe, dxo), (dwe, dwo) = P.gated_grad(xe, we, "silu", dh, dtype)
+    both = xe @ we.T
+    a, da = P.activation("silu", both[:, :f])
+    ed = 1.1 * np.concatenate([edh * np.abs(both[:, f:] * da), edh * np.abs(a)], 1) + 1e-5 * np.tile(edh, 2)      # (errors of a, da and up on top of edh's: far below a tenth)
+    _check(_got(dx), dxe, dxo + ed @ np.abs(we), dtype, "dx")
+    _check(_got(dw), dwe, dwo + ed.T @ np.abs(xe), dtype, "dw_in")
+
+
+def test_a_feed_forward_layer_in_bfloat16_does_not_drift(gpu):
+    """Truncated results are half a unit too small on average; rounded to nearest their errors cancel, also in the gradients."""
+    rng = np.random.default_rng(8)
+    (x, xe), (w, we), (o, oe), (g, ge) = (_make(rng, s, "bfloat16", c) for s, c in (((256, 64), 1.0), ((128, 64), 0.2), ((96, 64), 0.3), ((256, 96), 1.0)))
+    h = jt.nn.gated_linear(x, w)
+    y = jt.nn.gated_ffn(x, w, o)
+    do = jt.grad((y * g).sum(), o)
+    he = _got(h)
+    for got, want in ((_got(y), he @ oe.T), (_got(do), ge.T @ he)):
+        unit = 2.0 ** (np.floor(np.log2(np.abs(want))) - 7)
+        # the mean of n errors, even over half a unit to either side, has a deviation of 0.29 / sqrt(n); truncated results are at -0.5
+        assert abs(((np.abs(got) - np.abs(want)) / unit).mean()) < 6 * 0.29 / np.sqrt(want.size)
+
+
 @pytest.mark.parametrize("m,k,n,ta,tb", [(40, 30, 20, 0, 0), (256, 512, 256, 0, 1), (512, 256, 512, 1, 0), (64, 4096, 64, 1, 0), (7, 33, 9, 0, 1), (9300, 1024, 2048, 1, 0), (9300, 1024, 2048, 0, 0)])
 def test_products_rounded_to_nearest(gpu, m, k, n, ta, tb):
     """mjt_matmul_nearest on each of the product kernels' routes: whole, in slices, plain."""

@@ -372,3 +372,42 @@ def test_a_result_that_was_asked_for_twice_is_made_twice(launches):
     jt.sync([y] + again)
     assert y._op is None and all(v._op is None and v._buf is not None for v in again)
     assert sorted(launches) == [("gated_linear", [0, 1]), ("gated_linear", [1])]
+
+
+def test_a_feed_forward_layer_in_bfloat16_is_rounded_to_nearest_throughout(launches):
+    """Its second product and that product's gradients are the operators' own, not the ordinary product, which truncates."""
+    x, w, o = (core.Var(list(n), "bfloat16") for n in ((3, 5, 8), (12, 8), (7, 6)))
+    for v in (x, w, o):
+        v._buf = core.Buffer(2 * v.num)
+    y = jt.nn.gated_ffn(x, w, o)
+    grads = jt.grad((y * 2.0).sum(), [x, w, o])
+    assert [g.shape for g in [y] + grads] == [[3, 5, 7], [3, 5, 8], [12, 8], [7, 6]] and {g.dtype for g in [y] + grads} == {"bfloat16"}
+    jt.sync([y] + grads)
+    assert sorted(launches) == [("gated_linear", [0, 1]), ("gated_linear_grad", [0])] + 5 * [("product", [0])]
+    with pytest.raises(ValueError):
+        jt.nn.gated_ffn(x, w, _x(7, 5, dtype="bfloat16"))
+
+
+@pytest.mark.parametrize("trans_a,trans_b", [(False, False), (False, True), (True, False)])
+def test_gradients_of_a_product_are_products(trans_a, trans_b):
+    """sum(dc * A' B') moves with a and b as the products that are taken for its gradients say."""
+    rng = np.random.default_rng(4)
+    m, n, k = 3, 4, 5
+    shapes = [(k, m) if trans_a else (m, k), (n, k) if trans_b else (k, n), (m, n)]
+    values = {}
+
+    def var(shape):
+        v = _x(*shape)
+        values[v.id] = rng.standard_normal(shape)
+        return v
+
+    def times(a, b, ta, tb):
+        return (a.T if ta else a) @ (b.T if tb else b)
+
+    a, b, dc = map(var, shapes)
+    c = layers._result(layers.Call("product", trans_a, trans_b), 0, [a, b], [m, n], "float32")
+    got = [times(*(values[u.id] for u in g._op.inputs), *g._op.call.options) for g in layers._product_gradients(c._op, [a, b], {0: dc}, [True, True])]
+    for i, (v, g) in enumerate(zip((a, b), got)):
+        along = rng.standard_normal(v.shape)
+        moved = [along if j == i else values[u.id] for j, u in enumerate((a, b))]
+        assert abs((times(*moved, trans_a, trans_b) * values[dc.id]).sum() - (g * along).sum()) < 1e-12
