@@ -379,7 +379,7 @@ int mjt_init(int device) {
         if (device == -1) {
             // compile-only mode: no device is touched
             memset(&c.prop, 0, sizeof(c.prop));
-            strcpy(c.prop.gcnArchName, "gfx950");
+            strcpy(c.prop.gcnArchName, "gfx950:sramecc+:xnack-");   // as an MI355X names itself: what is cached here is found there
             c.prop.multiProcessorCount = 256;
             c.device = -1;
             c.dry_run = true;
