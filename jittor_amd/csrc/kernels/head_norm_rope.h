@@ -54,6 +54,12 @@ __device__ __forceinline__ float mjt_row_sum(float v) {
     for (int off = 16; off < LP; off *= 2) v += __shfl_xor(v, off, 64);
     return v;
 }
+// (the instruction takes a subnormal number for zero: without eps, rows of elements below 1e-19)
+__device__ __forceinline__ float mjt_rsqrt(float v) {
+    const bool low = v < 0x1p-96f;
+    const float r = __builtin_amdgcn_rsqf(low ? v * 0x1p64f : v);
+    return low ? r * 0x1p32f : r;
+}
 template <int I> struct mjt_ic { static constexpr int v = I; };
 template <int I, int N, class F> __device__ __forceinline__ void mjt_each(F&& f) {
     if constexpr (I < N) {
@@ -240,7 +246,7 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
                 }
                 sum += in[c] ? mine : 0.0f;
             }
-            const float r = NORM ? __builtin_amdgcn_rsqf(mjt_row_sum(sum) * (1.0f / D) + eps) : 1.0f;
+            const float r = NORM ? mjt_rsqrt(mjt_row_sum(sum) * (1.0f / D) + eps) : 1.0f;
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll

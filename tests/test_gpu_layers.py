@@ -297,6 +297,23 @@ def test_heads_that_are_zero_or_not_finite(gpu):
     assert np.array_equal(q, q1) and np.array_equal(k, k1)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("size", [1e-18, 1e-19, 1e-20])
+def test_heads_whose_mean_square_is_subnormal(gpu, dtype, size):
+    """Without eps.  Squares, their sum and its mean are each within half the least subnormal number, 2^-150, or E of their size; r has half the
+    relative error of the mean."""
+    rng = np.random.default_rng(31)
+    (x, xe), (s, se), (g, ge) = _make(rng, (1, 5, 3, 64), dtype, size), _make(rng, (64,), dtype, 0.2, 1.0), _make(rng, (1, 5, 3, 64), dtype)
+    y = jt.nn.head_norm_rope(x, s, eps=0.0)
+    dx = jt.grad((y * g).sum(), x)
+    mean = (xe[0] ** 2).mean(-1, keepdims=True)
+    off = 64 * E + 3 * 2.0 ** -150 / mean
+    want = P.head_norm(xe[0], se, None, None, 0.0, False)
+    _check(_got(y)[0], want, off * np.abs(want), dtype, "y")
+    want, _, sizes, _ = P.head_norm_grad(xe[0], se, None, None, 0.0, False, ge[0])
+    _check(_got(dx)[0], want, 4 * off * sizes, dtype, "dx")
+
+
 def test_positions_outside_the_table_make_nan_of_what_they_turn(gpu):
     rng = np.random.default_rng(9)
     x, g = (jt.array(rng.standard_normal((1, 5, 3, 16)).astype(np.float32)) for _ in range(2))
