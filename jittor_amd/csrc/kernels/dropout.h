@@ -8,9 +8,10 @@
 // for one pass in 128 (never where T's lower half is 0, p = 0.5 or 0.25): full resolution of p for half the arithmetic.
 // A dropped element is 0 whatever it held, also an infinity or NaN.
 //
-// Supplied by the host: TYPE (element type), RES, WIDE (a lane's eight elements are whole aligned vectors), STREAMS.
-// a[0] x  a[1] residual  a[2] y  a[3] elements  a[4] key  a[5] call  a[6] T  a[7] 1 / (1 - p) (double bits)  a[8] the side, in place in the counter's second word
-struct Params { void* a[9]; };
+// Supplied by the host: TYPE (element type), RES, WIDE (a lane's eight elements are whole aligned vectors), SIDE (in place in the counter's second
+// word, which no element's place reaches there), STREAMS.  (As a parameter the side took 3 of 61 us of the case of 8192 x 4096 bfloat16 with a residual.)
+// a[0] x  a[1] residual  a[2] y  a[3] elements  a[4] key  a[5] call  a[6] T  a[7] 1 / (1 - p) (double bits)
+struct Params { void* a[8]; };
 
 struct mjt_u4 { unsigned w[4]; };
 // ten rounds of two multiplications of 32 bits to 64 and the key's Weyl steps
@@ -30,10 +31,10 @@ __device__ __forceinline__ mjt_u4 mjt_philox(unsigned c0, unsigned c1, unsigned 
 __device__ __forceinline__ unsigned mjt_half_of(const mjt_u4& w, int j) { return j & 1 ? w.w[j / 2] >> 16 : w.w[j / 2] & 0xffffu; }
 
 // bit j: element j of group g is kept
-__device__ __forceinline__ unsigned mjt_keep_bits(unsigned long long g, unsigned long long key, unsigned long long call, unsigned long long threshold, unsigned side) {
+__device__ __forceinline__ unsigned mjt_keep_bits(unsigned long long g, unsigned long long key, unsigned long long call, unsigned long long threshold) {
     const unsigned hi = (unsigned)(threshold >> 16), lo = (unsigned)(threshold & 0xffffu);        // hi up to 65536, for p = 1
     const unsigned k0 = (unsigned)key, k1 = (unsigned)(key >> 32), c2 = (unsigned)call, c3 = (unsigned)(call >> 32);
-    const mjt_u4 a = mjt_philox((unsigned)g, (unsigned)(g >> 32) | side, c2, c3, k0, k1);
+    const mjt_u4 a = mjt_philox((unsigned)g, (unsigned)(g >> 32) | SIDE, c2, c3, k0, k1);
     unsigned keep = 0, tie = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -42,7 +43,7 @@ __device__ __forceinline__ unsigned mjt_keep_bits(unsigned long long g, unsigned
         tie |= (u == hi ? 1u : 0u) << j;
     }
     if (lo != 0 && __any(tie != 0)) {
-        const mjt_u4 b = mjt_philox((unsigned)g, (unsigned)(g >> 32) | side | 0x80000000u, c2, c3, k0, k1);
+        const mjt_u4 b = mjt_philox((unsigned)g, (unsigned)(g >> 32) | SIDE | 0x80000000u, c2, c3, k0, k1);
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if ((tie >> j & 1) && mjt_half_of(b, j) < lo) keep &= ~(1u << j);
@@ -71,7 +72,7 @@ extern "C" __global__ __launch_bounds__(256) void ENTRY(Params p) {
                 if (RES) add.v[j] = j < have ? res[g * 8 + j] : raw(0);
             }
         }
-        const unsigned keep = threshold ? mjt_keep_bits((unsigned long long)g, key, call, threshold, (unsigned)(unsigned long long)p.a[8]) : 0xffu;
+        const unsigned keep = threshold ? mjt_keep_bits((unsigned long long)g, key, call, threshold) : 0xffu;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             float v = keep >> j & 1 ? mjt_el<TYPE>::up(in.v[j]) * scale : 0.0f;
