@@ -19,7 +19,7 @@
 // training step, whose other tensors leave less of these in the caches): a row of 80 keeps ten of sixteen lanes busy, and arithmetic bounds its gradient.
 //
 // Supplied by the host: TYPE, STYPE (types of x and of the scales), D, ROT, V, LP, NC, IT, PAIRED, FIRST, NORM, STREAMS, AXES, ENDS, POS (positions are
-// given), SUBNORMAL (eps is below the normal numbers), BACK, SUMS (BACK with gradients of the scales).
+// given), BACK, SUMS (BACK with gradients of the scales).
 // a[0] x  a[1] q  a[2] k  a[3] v  (BACK: dq, dk, dv, null where missing; forward: null where not wanted)  a[4] scale of q  a[5] of k  a[6] table  a[7] positions
 // a[8] tokens  a[9] tokens of a sequence  a[10] HQ  a[11] HK  a[12] HV  a[13] eps (double bits)  a[14] positions of an axis  a[15] rows of the table
 // a[16] dx  a[17] partial sums [workgroup][2][D]
@@ -54,10 +54,8 @@ __device__ __forceinline__ float mjt_row_sum(float v) {
     for (int off = 16; off < LP; off *= 2) v += __shfl_xor(v, off, 64);
     return v;
 }
-// The instruction takes a subnormal number for zero: without eps, rows of elements below 1e-19 (SUBNORMAL 1; with a normal eps nothing is that small, and the
-// four operations a row took 1.2 of qkv's 38.5 us at 8192 tokens of 48 heads of 128 bfloat16).
+// (the instruction takes a subnormal number for zero: without eps, rows of elements below 1e-19)
 __device__ __forceinline__ float mjt_rsqrt(float v) {
-    if (!SUBNORMAL) return __builtin_amdgcn_rsqf(v);
     const bool low = v < 0x1p-96f;
     const float r = __builtin_amdgcn_rsqf(low ? v * 0x1p64f : v);
     return low ? r * 0x1p32f : r;

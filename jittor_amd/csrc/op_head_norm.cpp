@@ -125,7 +125,7 @@ Plan plan_for(const char* who, const mjt_tensor* x, const mjt_tensor* q_scale, c
     std::ostringstream defs;
     defs << "#define STREAMS " << (far ? 1 : 0) << "\n#define TYPE " << a.type << "\n#define STYPE " << a.scale_type << "\n#define D " << D << "\n#define ROT " << rot << "\n#define V " << V << "\n#define LP " << LP << "\n#define NC " << NC
          << "\n#define PAIRED " << (p->interleaved ? 1 : 0) << "\n#define FIRST " << (p->heads_first ? 1 : 0) << "\n#define NORM " << (q_scale ? 1 : 0) << "\n#define AXES " << axes
-         << "\n#define ENDS " << ends << "\n#define POS " << (positions ? 1 : 0) << "\n#define SUBNORMAL " << ((float)p->eps < 0x1p-126f ? 1 : 0) << "\n";
+         << "\n#define ENDS " << ends << "\n#define POS " << (positions ? 1 : 0) << "\n";
     a.defines = defs.str();
     a.name = std::string("mjt_head_norm_rope_") + mjt_dtype_name(x->dtype) + "_" + std::to_string(D) + (far ? "_streams" : "");
     auto ptr = [](const mjt_tensor* t) { return bits_of_ptr(t ? t->ptr : nullptr); };
