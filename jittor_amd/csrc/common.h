@@ -202,24 +202,25 @@ std::string fused_op_expr(const mjt_fused_desc* d, const mjt_fused_op& o);
 inline uint64_t bits_of(double v) { uint64_t u; memcpy(&u, &v, 8); return u; }
 inline uint64_t bits_of_ptr(const void* p) { return (uint64_t)(uintptr_t)p; }
 
-// While one of these lives on this thread, products write bfloat16 results rounded to nearest even instead of truncated (op_matmul.cpp).
+// While one of these lives on this thread, products are those of layers' operators: bfloat16 results rounded to nearest even instead of truncated, rows of
+// any length as they lie, and tiles that other products, which keep the sums they had, do not take (op_matmul.cpp).
 struct Nearest {
     Nearest();
     ~Nearest();
     static bool on();
 };
 
-// Gated projections on the tiles of the general product kernel (op_matmul.cpp, kernels/gemm_mfma.h with GATED): rows of x and of the
-// weights [2 F, K] are whole 16-byte pieces that begin at one.  False, with nothing launched: the product is better cut into slices of its sum.
+// Gated projections on the tiles of the general product kernel (op_matmul.cpp, kernels/gemm_mfma.h with GATED): x [M, K] and the
+// weights [2 F, K], rows of any length.  False, with nothing launched: the product is better cut into slices of its sum.
 bool gemm_gated(int dtype, int act, const char* act_name, const void* x, const void* w, void* y, void* both, int64_t M, int64_t F, int64_t K);
 
 // ---- operators of transformer layers (op_layers.cpp) ----
 // The number of a float type inside kernels/element.h, -1 for other types.
 int element_type(int dtype);
-// The kernel `name` made of embedded source files behind `defines`, built once; its launcher is called for every launch, so the key is
-// all there is to look up.
 // Whether a kernel that passes over `bytes` once reads and writes past the caches (element.h).
 inline bool streams(int64_t bytes) { return bytes >= (int64_t(32) << 20); }
+// The kernel `name` made of embedded source files behind `defines`, built once; its launcher is called for every launch, so the key is
+// all there is to look up.
 JitKernel* layer_kernel(const std::string& name, std::initializer_list<const char*> files, const std::string& defines);
 
 // Threads of a workgroup of kernels/gemm_mfma.h, with float32 operands in parts or as they are.

@@ -7,15 +7,15 @@
 // load and the odd ones in another, and is multiplied with both: of the results of the even parts the first eight rows count, of the odd ones the
 // others, and the two halves of a wave add them up.  Half of the products are thrown away; the matrix units have time.  (A piece of 64 bytes of each of the
 // sixteen rows of g and u a load, every product used: lines come in halves, which loads past the caches pay for twice; us so / now, one row of x and weights that are
-// not in the caches: 4096 -> 11264 37.3 / 32.9, 5120 -> 13824 55.1 / 45.8, 2560 -> 6912 20.0 / 15.6.)
+// not in the caches: 4096 -> 11264 37.3 / 32.4, 5120 -> 13824 55.1 / 44.8, 2560 -> 6912 20.0 / 15.4.)
 // float32: the products take four times as long, so the rows of g and of u are the sixteen rows of one operand and every product counts; a load is 64
 // bytes of each row, through the caches, where the other half of the line waits for the next (4096 -> 4096 27.3 us, 30.8 past them).  A lane's four k feed four MFMAs of 4 k each; both
 // operands use the same pairing.
 // The waves' sums meet in LDS, where gate and up of a result meet too.
 //
-// us a call over weights that are not in the caches, floor at the rate of a large copy (5.19 TB/s; reads alone are faster): bfloat16 1 x 4096 -> 11264 32.8, 35.6; 1 x 5120 -> 13824
-// 48.3, 54.6; 8 x 2048 -> 5632 12.0, 8.9; 1 x 8192 -> 1024, 128 workgroups on 256 units, 14.4, 6.5; float32 1 x 2048 -> 8192 24.8, 25.9.  With sixteen rows of g and of u a
-// workgroup half as many workgroups leave some compute units with twice the others' work.  More rows of x wait for x: 16 x 4096 -> 11264 48.4; those go to tiles.
+// us a call over weights that are not in the caches, floor at the rate of a large copy (5.19 TB/s; reads alone are faster): bfloat16 1 x 4096 -> 11264 32.4, 35.6; 1 x 5120 -> 13824
+// 44.8, 54.6; 8 x 2048 -> 5632 12.7, 8.9; 1 x 8192 -> 1024, 128 workgroups on 256 units, 15.9, 6.5; float32 1 x 2048 -> 8192 24.2, 25.9.  With sixteen rows of g and of u a
+// workgroup half as many workgroups leave some compute units with twice the others' work.  More rows of x wait for x: 16 x 4096 -> 11264 46.0; those go to tiles.
 //
 // Supplied by the host: TYPE, ACT, W, UN, BOTH (gate and up are wanted), Y (y is wanted), RAGGED (otherwise rows of x
 // and of the weights are multiples of 16 bytes and begin at one).  Rows past the last are read from the last, their results are not stored.

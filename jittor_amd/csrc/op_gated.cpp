@@ -38,8 +38,8 @@ void rows_pass(int act, const void* both, const void* y, const void* d, int dtyp
 
 // The ways to run the projections, by estimated time.
 //   FEW (kernels/gated_few.h): up to 8 rows, and up to 16 where x is not the longer way: float32, whose MFMAs of other routes wait as well, and up to 48 MB of 16-bit weights
-//   (us few / MFMA or TILES, weights not in the caches: bfloat16 8 x 4096 -> 11264 39.3 / 41.4, 8 x 2048 -> 5632 12.0 / 15.2, 16 x 2048 -> 5632 14.1 / 15.4, on the other side 16 x 4096 ->
-//   11264 48.4 / 42.3, 16 x 2560 -> 6912 22.8 / 18.5; float32 16 x 4096 -> 4096 38.7 / 42.5).  Rows that are no whole 16-byte pieces, whose loads cross lines: 16 bits up to 20 MB,
+//   (us few / MFMA or TILES, weights not in the caches: bfloat16 8 x 4096 -> 11264 39.7 / 45.9, 8 x 2048 -> 5632 12.7 / 15.3, 16 x 2048 -> 5632 14.2 / 15.2, on the other side 16 x 4096 ->
+//   11264 46.0 / 45.5, 16 x 2560 -> 6912 22.6 / 18.0; float32 16 x 4096 -> 4096 38.4 / 45.7; more sizes in profiles/gated_routes.txt).  Rows that are no whole 16-byte pieces, whose loads cross lines: 16 bits up to 20 MB,
 //   float32 up to 8 rows or 48 MB (bfloat16 4 x 1501 -> 1500 9.7 / 12.3, 4 x 2231 -> 2610 22.3 / 16.7; float32 4 x 4001 -> 9001 84.8 / 98.3, 16 x 4001 -> 9001 114.7 / 99.8).
 //   TILES (kernels/gemm_dma.h): 16-bit operands on 256 x 256 tiles, one to a compute unit, or 128 x 128, two to a unit.  Up to 128 rows only the latter (128 x 8192 -> 28672 235 /
 //   188), up to 64 none: MFMA has tiles of 64 rows (us TILES / MFMA: 64 x 5120 -> 13824 62.9 / 57.5, 64 x 1536 -> 8960 20.1 / 18.9, 24 x 4096 -> 11264 42.2 / 42.1).
@@ -48,8 +48,9 @@ void rows_pass(int act, const void* both, const void* y, const void* d, int dtyp
 //   float32 3722 x 99 -> 3968 135 / 101, 1024 x 513 -> 1377 45.5 / 30.2).
 // A stage of 64 elements of the sum takes 1.1 us on a 256 x 256 tile, 0.33 on a 128 x 128 tile with a unit to itself and 0.66 for two of them (more
 // where the sum is long and neighbours drift apart), 0.25 on a 64 x 64 tile; a round begins with the first loads and ends with the
-// activations and stores, 10, 6 and 3.5 us.  Rows that are no whole 128-byte lines cost a quarter more.
-// us measured 256 / 128 / MFMA for bfloat16: 64 x 2048 -> 5632 43 / 16.3 / 11.3; 256 x 2048 -> 5632 45 / 17.5 / 22.4; 1024 x 2048 -> 5632 49.7 / 54.5 / 54.4; 2048 x
+// activations and stores, 10, 6 and 3.5 us; a further round of tiles whose sum is long, a fifth more.  Left out: rows that are
+// no whole 128-byte lines cost a quarter more on tiles, and weights that are not in the caches 5 us on tiles of 128 (80 to 128 rows would be MFMA's then).
+// us measured 256 / 128 / MFMA for bfloat16, weights in the caches where they fit: 64 x 2048 -> 5632 43 / 16.3 / 11.3; 256 x 2048 -> 5632 45 / 17.5 / 22.4; 1024 x 2048 -> 5632 49.7 / 54.5 / 54.4; 2048 x
 // 2048 -> 5632 103.6 / 92.4 / 106; 8192 x 2048 -> 5632 335 / 367 / 393; 512 x 4096 -> 11264 107 / 134 / 106; 777 x 1000 -> 2600 34.5 / 22.8 / 25.8; 512 x 1024 -> 2816
 // 28.5 / 11.5 / 13.9; 4096 x 512 -> 1376 23.0 / 20.2 / 24.1.
 enum Route { FEW, TILES, MFMA, PRODUCT };
@@ -80,7 +81,7 @@ Route choose(int dtype, int64_t M, int64_t F, int64_t K, bool aligned, int* tile
 void few_rows(const mjt_tensor* x, const mjt_tensor* w, int act, const mjt_tensor* y, const mjt_tensor* both) {
     const int64_t M = x->shape[0], K = x->shape[1], F = w->shape[0] / 2;
     // Lines of 128 bytes that a wave takes at a time: the most for which every wave has the same number of runs (us for 1 / 2 / 4, bfloat16, one row, weights not in
-    // the caches: 4096 -> 11264 34.4 / 34.1 / 32.2, 4096 -> 14336 45.6 / 44.8 / 38.3, 5120 -> 13824 48.0 / 44.1 / 46.2, 2560 -> 6912 14.5 / 14.7 / 15.9, 1536 -> 8960 11.6 / 11.8 / 13.0).
+    // the caches: 4096 -> 11264 34.4 / 34.1 / 32.2, 4096 -> 14336 45.6 / 44.8 / 38.3, 5120 -> 13824 48.0 / 44.1 / 46.2, 2560 -> 6912 14.5 / 14.7 / 15.9 (15.4 another time), 1536 -> 8960 11.6 / 11.8 / 13.0).
     // Four waves instead of eight: 37.9 / 36.0 / 37.3 for the first of these, 8192 -> 1024 20.3 instead of 12.6.
     const int W = 8;
     const int64_t turn = W * 128 / dtype_size(x->dtype);

@@ -228,7 +228,8 @@ def dropout(x, p=0.5, is_train=False, seed=None, offset=None, residual=None):
 
     The mask is never stored: it depends on the elements' places, `seed` and `offset` (integers of 64 bits) alone, and the gradient works
     it out again.  Calls of one program that are to be independent differ in one of the two; without a seed the generator of jt.set_seed
-    numbers the calls, whose numbers no seed and offset give.  A dropped element is 0 whatever it held."""
+    numbers the calls, whose numbers no seed and offset give.  A dropped element is 0 whatever it held.  `p` belongs to the graph: where it changes from step to step,
+    each value's first step is worked out anew; seeds and offsets may change."""
     return layers.dropout(x, p, is_train, seed, offset, residual)
 
 
@@ -265,7 +266,12 @@ def head_norm_rope(x, scale=None, table=None, positions=None, sections=None, eps
 
 def gated_linear(x, weight, activation="silu"):
     """activation(x * g^T) * (x * u^T) for weight [2 f, k] = g above u: the first half of a gated feed-forward layer, both projections and
-    what follows them in one pass.  `activation`: silu, gelu, relu or sigmoid."""
+    what follows them in one pass.  `activation`: silu, gelu, relu or sigmoid.
+
+    Gradients read the two products in float32, 8 bytes for each element of the result, from the forward pass on where both are computed together; after a forward
+    pass computed by itself, and for gradients that are computed one after the other, the products are made again.  In 16 bits the gradient
+    of the two products is rounded to x's type, as the operands of the products behind it have to be (the error of dx and dw is 1.4 times that of results
+    rounded once; x and weight cast to float32 have neither rounding).  Second derivatives are refused."""
     return layers.gated_linear(x, weight, activation)
 
 
