@@ -3,7 +3,7 @@
 Most of a GPU test's time is the run-time compiler's, one kernel after the other (0.2 s each, some 4000 in all).  A run of many GPU tests
 therefore starts helpers, each with every n-th chunk of the same tests in compile-only mode: results are zeros, assertions are off, and
 what is left of a test are its kernels, which land in the cache on disk that the run itself looks into.  A helper that fails costs the run nothing
-but time.  No helper touches the device."""
+but time."""
 import ctypes
 import os
 import signal
@@ -14,6 +14,7 @@ import tempfile
 import numpy as np
 
 HELPERS, CHUNK, FEWEST = 10, 8, 100
+_lists = []
 _VARIABLE = "MJT_TESTS_AHEAD"                                # "number of the helper/helpers/file with the names of the tests"
 
 
@@ -29,7 +30,8 @@ def start(items, root):
         return []
     with tempfile.NamedTemporaryFile("w", suffix=".txt", delete=False) as f:
         f.write("\n".join(names))
-    env = dict(os.environ, OMP_NUM_THREADS="1", OPENBLAS_NUM_THREADS="1")
+    _lists.append(f.name)
+    env = dict(os.environ, OMP_NUM_THREADS="1", OPENBLAS_NUM_THREADS="1", HIP_VISIBLE_DEVICES="-1")      # (no helper sees a device)
     env.pop("PYTEST_ADDOPTS", None)
     command = [sys.executable, "-O", "-m", "pytest", "--assert=plain", "-p", "no:cacheprovider", "-q", "-m", "gpu", os.path.join(root, "tests")]
     return [subprocess.Popen(command, cwd=root, env=dict(env, **{_VARIABLE: "%d/%d/%s" % (i, n, f.name)}), stdin=subprocess.DEVNULL, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
@@ -41,6 +43,8 @@ def stop(helpers):
         p.kill()
     for p in helpers:
         p.wait()
+    while _lists:
+        os.unlink(_lists.pop())
 
 
 def become_helper():
